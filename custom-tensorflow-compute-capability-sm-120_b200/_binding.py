@@ -72,6 +72,29 @@ class SM120GemmDesc(Structure):
     ]
 
 
+class SM120ScoreAttentionDesc(Structure):
+    """Field-for-field image of ``struct SM120ScoreAttentionDesc``."""
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("dtype", c_int32),
+        ("causal", c_int32),
+        ("num_documents", c_int32),
+        ("batch", c_int64), ("heads", c_int64), ("kv_heads", c_int64), ("seq_q", c_int64), ("seq_k", c_int64), ("head_dim", c_int64),
+        ("scale", c_float), ("softcap", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("alibi_slopes", c_void_p), ("document_offsets", c_void_p), ("prefix_lengths", c_void_p),
+        ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("out_stride", c_int64 * 3),
+        ("grad_out", c_void_p), ("grad_q", c_void_p), ("grad_k", c_void_p), ("grad_v", c_void_p),
+        ("grad_out_stride", c_int64 * 3), ("grad_q_stride", c_int64 * 3), ("grad_k_stride", c_int64 * 3), ("grad_v_stride", c_int64 * 3),
+        ("key_lengths", c_void_p), ("prefix_k", c_void_p), ("prefix_v", c_void_p),
+        ("prefix_len", c_int64),
+        ("prefix_k_stride", c_int64 * 2), ("prefix_v_stride", c_int64 * 2),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_uint64),
+        ("stream", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes): every symbol the public header declares
 EXPORTS = {
     "sm120_launch_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_int, c_void_p]),
@@ -98,6 +121,12 @@ EXPORTS = {
     "sm120_launch_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_int, c_void_p]),
     "sm120_launch_attention_ex": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                           c_float, c_int, c_int, c_void_p]),
+    "sm120_score_attention_desc_init": (None, [POINTER(SM120ScoreAttentionDesc)]),
+    "sm120_launch_score_attention": (c_int, [POINTER(SM120ScoreAttentionDesc)]),
+    "sm120_score_attention_grad_workspace_bytes": (ctypes.c_size_t, [POINTER(SM120ScoreAttentionDesc)]),
+    "sm120_launch_score_attention_grad": (c_int, [POINTER(SM120ScoreAttentionDesc)]),
+    "sm120_score_attention_decode_workspace_bytes": (ctypes.c_size_t, [POINTER(SM120ScoreAttentionDesc)]),
+    "sm120_launch_score_attention_decode": (c_int, [POINTER(SM120ScoreAttentionDesc)]),
     "sm120_launch_bias_grad": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
     "sm120_is_supported": (c_bool, [c_int]),
     "sm120_get_error_string": (c_char_p, [c_int]),
@@ -149,6 +178,12 @@ def library_loaded() -> bool:
 def new_desc() -> SM120GemmDesc:
     d = SM120GemmDesc()
     load_library().sm120_gemm_desc_init(ctypes.byref(d))
+    return d
+
+
+def new_score_attention_desc() -> SM120ScoreAttentionDesc:
+    d = SM120ScoreAttentionDesc()
+    load_library().sm120_score_attention_desc_init(ctypes.byref(d))
     return d
 
 

@@ -84,6 +84,19 @@ cudaError_t query_device(int device, int* sm_count) {
     return cudaSuccess;
 }
 
+}  // namespace
+
+cudaError_t current_device(int* device, int* sm_count) {
+    const cudaError_t e = cudaGetDevice(device);
+    return e != cudaSuccess ? e : query_device(*device, sm_count);
+}
+uint64_t launch_wait_limit_ns() { return wait_limit_ns(); }
+void note_launches(const char* name, int count) {
+    g_launch_count.fetch_add(static_cast<uint64_t>(count), std::memory_order_relaxed);
+    t_last_kernel = name;
+}
+
+namespace {
 bool valid_dtype(int d) { return d >= SM120_DTYPE_FLOAT32 && d <= SM120_DTYPE_FP8_E4M3; }
 
 // Checks every field that can be checked without touching the device and

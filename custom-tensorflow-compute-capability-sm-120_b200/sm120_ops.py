@@ -805,6 +805,316 @@ def flash_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Ten
                                         attention_mask=attention_mask, causal_mask=causal_mask, return_attention_scores=True)
 
 
+# ---------------------------------------------------------------------------
+# attention with modified scores: prompts, gradients, next tokens
+# ---------------------------------------------------------------------------
+_SCORE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check_same(name: str, t, like: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{name} must have the query's dtype {like.dtype}, got {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the query on {like.device}")
+
+
+def _check_side(name: str, t, shape, dtype: torch.dtype, like: torch.Tensor) -> None:
+    """A small companion tensor (slopes, offsets, lengths, lse): exact shape and dtype, contiguous, on the query's device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise InvalidArgumentError(f"{name} must be a {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the query on {like.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _score_operand(t: torch.Tensor) -> torch.Tensor:
+    """`t` as the tensor-core kernels can address it: contiguous head dimension, and for 16-bit types 16-byte aligned
+    with strides that are multiples of 16 bytes.  Other layouts are copied once."""
+    strides = t.stride()
+    if strides[-1] != 1 and t.shape[-1] != 1:
+        return t.contiguous()
+    if t.dtype != torch.float32 and t.shape[-1] % 8 == 0 and t.shape[-1] <= 128:
+        if t.data_ptr() % 16 or any(st % 8 or (st == 0 and e > 1) for st, e in zip(strides[:-1], t.shape[:-1]) if e != 1):
+            c = t.contiguous()
+            return c.clone(memory_format=torch.contiguous_format) if c.data_ptr() % 16 else c
+    return t
+
+
+def _score_options(query: torch.Tensor, heads: int, scale: Optional[float], softcap: Optional[float], alibi_slopes) -> _b.SM120ScoreAttentionDesc:
+    d = _b.new_score_attention_desc()
+    d.dtype = _TORCH_TO_SM120[query.dtype]
+    d.head_dim = query.shape[-1]
+    d.scale = 1.0 / float(query.shape[-1]) ** 0.5 if scale is None else float(scale)
+    if d.scale != d.scale:
+        raise ValueError("scale must not be NaN")
+    if softcap is not None:
+        if not (0.0 < float(softcap) <= 1e30):
+            raise ValueError(f"softcap must be positive (None switches it off), got {softcap}")
+        d.softcap = float(softcap)
+    if alibi_slopes is not None:
+        _check_side("alibi_slopes", alibi_slopes, (heads,), torch.float32, query)
+        d.alibi_slopes = alibi_slopes.data_ptr()
+    return d
+
+
+def _set_strides(d, name: str, t: torch.Tensor, count: int = 3) -> None:
+    getattr(d, name)[:] = t.stride()[:count]
+
+
+def _score_sequence_desc(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths):
+    """Checks the arguments of the sequence forms and fills a descriptor but for what is written; returns it with the operands it points to."""
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a tensor")
+    if query.dtype not in _SCORE_DTYPES:
+        raise ValueError(f"dtype {query.dtype} is not supported (float32, float16, bfloat16)")
+    _check_same("key", key, query)
+    _check_same("value", value, query)
+    if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
+        raise ValueError("query, key and value must be 4-dimensional [batch, heads, seq, head_dim]")
+    b, h, sq, dim = query.shape
+    kv_heads, sk = key.shape[1], key.shape[2]
+    if tuple(key.shape) != (b, kv_heads, sk, dim) or tuple(value.shape) != (b, kv_heads, sk, dim):
+        raise InvalidArgumentError("query [B, H, Sq, D], key [B, Hk, Sk, D] and value [B, Hk, Sk, D] are required")
+    if h < 1 or kv_heads < 1 or h % kv_heads:
+        raise InvalidArgumentError(f"the number of query heads ({h}) must be a multiple of the number of key heads ({kv_heads})")
+    if not 1 <= dim <= 256:
+        raise InvalidArgumentError(f"head dimension {dim} is not supported (1 to 256)")
+    d = _score_options(query, h, scale, softcap, alibi_slopes)
+    d.causal = int(bool(causal_mask))
+    d.batch, d.heads, d.kv_heads, d.seq_q, d.seq_k = b, h, kv_heads, sq, sk
+    if document_offsets is not None:
+        if prefix_lengths is not None:
+            raise InvalidArgumentError("document_offsets and prefix_lengths cannot be combined")
+        if not isinstance(document_offsets, torch.Tensor) or document_offsets.dim() != 2 or document_offsets.shape[1] < 2:
+            raise InvalidArgumentError(f"document_offsets must have shape [{b}, documents + 1]")
+        _check_side("document_offsets", document_offsets, (b, document_offsets.shape[1]), torch.int32, query)
+        d.num_documents = document_offsets.shape[1] - 1
+        d.document_offsets = document_offsets.data_ptr() or None
+    if prefix_lengths is not None:
+        if not causal_mask:
+            raise InvalidArgumentError("prefix_lengths widens the causal mask: causal_mask must be set")
+        _check_side("prefix_lengths", prefix_lengths, (b,), torch.int32, query)
+        d.prefix_lengths = prefix_lengths.data_ptr() or None
+    _require_available()
+    if not query.is_cuda:
+        raise TypeError("query, key and value must be CUDA tensors")
+    query, key, value = _score_operand(query), _score_operand(key), _score_operand(value)
+    d.q, d.k, d.v = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    _set_strides(d, "q_stride", query)
+    _set_strides(d, "k_stride", key)
+    _set_strides(d, "v_stride", value)
+    return d, query, key, value
+
+
+def _score_launch(entry: str, what: str, d, device: torch.device) -> None:
+    """Calls a descriptor-taking entry point on the current stream of `device`."""
+    d.stream = torch.cuda.current_stream(device).cuda_stream
+    fn = getattr(_b.load_library(), entry)
+    if device.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(d))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(d))
+    if rc == _b.CUDA_ERROR_INVALID_VALUE:
+        raise InvalidArgumentError(f"{what} rejected its arguments (cudaErrorInvalidValue)")
+    if rc != _b.CUDA_SUCCESS:
+        raise InternalError(f"{what} failed: {_b.error_string(rc)}")
+
+
+def _score_out(out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(query)
+    _check_same("out", out, query)
+    if out.shape != query.shape or (out.shape[-1] > 1 and out.stride(-1) != 1):
+        raise ValueError(f"`out` must have shape {tuple(query.shape)} and a contiguous head dimension")
+    return out
+
+
+def score_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: Optional[float] = None,
+                    causal_mask: bool = False, softcap: Optional[float] = None, alibi_slopes: Optional[torch.Tensor] = None,
+                    document_offsets: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None,
+                    return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Attention with the score changes and masks of language models
+    (``sm120_launch_score_attention``; ``scaled_dot_product_attention`` is the plain form).
+
+    query [B, H, Sq, D], key and value [B, Hk, Sk, D] with H a multiple of Hk: query head h
+    reads key head h // (H // Hk).  Any strides with a contiguous head dimension, e.g.
+    [B, S, H, D] storage seen through ``transpose(1, 2)``.  Query i stands at position
+    i + Sk - Sq.  The score of query position i and key j is
+
+        x = scale * <q, k>  (scale defaults to 1 / sqrt(D));  softcap * tanh(x / softcap) with ``softcap``;
+        minus alibi_slopes[h] * |i - j| with ``alibi_slopes`` (float32 [H]);
+
+    and a query sees the keys that every given mask leaves:
+
+        causal_mask        j <= i;
+        prefix_lengths     (int32 [B], with causal_mask) j <= i or j < prefix_lengths[b];
+        document_offsets   (int32 [B, documents + 1], ascending) both positions inside the same
+                           [offsets[d], offsets[d + 1]); positions outside every document see
+                           nothing and nothing sees them, and may hold any values.
+
+    A query that sees no key gets zeros.  The three integer and slope tensors stay on the
+    device: their values are not checked on the host.  ``return_lse`` adds the float32
+    [B, H, Sq] logarithm of the softmax denominators (-inf where no key is seen), which
+    ``score_attention_grad`` needs.  ``out`` receives the result.  The call itself is not
+    recorded by autograd (``score_attention_trainable`` is).
+
+    float16 / bfloat16 with D a multiple of 8 up to 128 run on the tensor cores; float32 and
+    other D up to 256 on a plain kernel."""
+    d, query, key, value = _score_sequence_desc(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths)
+    out = _score_out(out, query)
+    d.out = out.data_ptr()
+    _set_strides(d, "out_stride", out)
+    lse = None
+    if return_lse:
+        lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
+        d.lse = lse.data_ptr() or None
+    _score_launch("sm120_launch_score_attention", "score_attention", d, query.device)
+    return (out, lse) if return_lse else out
+
+
+def score_attention_grad(grad_out: torch.Tensor, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, out: torch.Tensor,
+                         lse: torch.Tensor, *, scale: Optional[float] = None, causal_mask: bool = False, softcap: Optional[float] = None,
+                         alibi_slopes: Optional[torch.Tensor] = None, document_offsets: Optional[torch.Tensor] = None,
+                         prefix_lengths: Optional[torch.Tensor] = None):
+    """Gradients (query, key, value) of ``score_attention`` called with the same operands and
+    options, from its result `out`, its `lse` and the result's gradient
+    (``sm120_launch_score_attention_grad``).  Key and value gradients are summed over the query
+    heads that share a key head, in a fixed order.  The slopes have no gradient."""
+    d, query, key, value = _score_sequence_desc(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths)
+    for name, t in (("grad_out", grad_out), ("out", out)):
+        _check_same(name, t, query)
+        if t.shape != query.shape:
+            raise InvalidArgumentError(f"{name} must have the query's shape {tuple(query.shape)}, got {tuple(t.shape)}")
+    _check_side("lse", lse, query.shape[:3], torch.float32, query)
+    out, grad_out = _score_operand(out), _score_operand(grad_out)
+    dq, dk, dv = torch.empty_like(query), torch.empty_like(key), torch.empty_like(value)
+    d.out, d.lse, d.grad_out = out.data_ptr(), lse.data_ptr() or None, grad_out.data_ptr()
+    d.grad_q, d.grad_k, d.grad_v = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    _set_strides(d, "out_stride", out)
+    _set_strides(d, "grad_out_stride", grad_out)
+    _set_strides(d, "grad_q_stride", dq)
+    _set_strides(d, "grad_k_stride", dk)
+    _set_strides(d, "grad_v_stride", dv)
+    # scratch from the caller's allocator for this call alone: two captured graphs, or two streams, never share it
+    need = int(_b.load_library().sm120_score_attention_grad_workspace_bytes(ctypes.byref(d)))
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=query.device)
+    d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+    _score_launch("sm120_launch_score_attention_grad", "score_attention_grad", d, query.device)
+    return dq, dk, dv
+
+
+class _ScoreAttentionFunction(torch.autograd.Function):
+    """``score_attention`` with ``score_attention_grad`` as its backward pass."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, options):
+        out, lse = score_attention(query, key, value, return_lse=True, **options)
+        ctx.save_for_backward(query, key, value, out, lse)
+        ctx.options = options
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        query, key, value, out, lse = ctx.saved_tensors
+        return (*score_attention_grad(grad_out, query, key, value, out, lse, **ctx.options), None)
+
+
+def score_attention_trainable(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: Optional[float] = None,
+                              causal_mask: bool = False, softcap: Optional[float] = None, alibi_slopes: Optional[torch.Tensor] = None,
+                              document_offsets: Optional[torch.Tensor] = None, prefix_lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``score_attention`` that torch autograd can differentiate once with respect to query, key and
+    value (as ``dense_trainable`` is for a Dense layer).  Capturing a backward pass into a CUDA graph follows
+    torch's rules: take the gradients with ``torch.autograd.grad`` inside the capture, or capture
+    ``score_attention`` and ``score_attention_grad`` themselves."""
+    return _ScoreAttentionFunction.apply(query, key, value, dict(
+        scale=scale, causal_mask=causal_mask, softcap=softcap, alibi_slopes=alibi_slopes, document_offsets=document_offsets,
+        prefix_lengths=prefix_lengths))
+
+
+def _score_token(what: str, query, prefix_key, prefix_value, key_cache, value_cache, lengths, scale, softcap, alibi_slopes, return_lse, out):
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a tensor")
+    if query.dtype not in _SCORE_DTYPES:
+        raise ValueError(f"dtype {query.dtype} is not supported (float32, float16, bfloat16)")
+    _check_same("key_cache", key_cache, query)
+    _check_same("value_cache", value_cache, query)
+    if query.dim() != 3 or key_cache.dim() != 4 or value_cache.dim() != 4:
+        raise ValueError("query must be [batch, heads, head_dim], the caches [batch, key heads, seq, head_dim]")
+    b, h, dim = query.shape
+    kv_heads, sk = key_cache.shape[1], key_cache.shape[2]
+    if tuple(key_cache.shape) != (b, kv_heads, sk, dim) or tuple(value_cache.shape) != (b, kv_heads, sk, dim):
+        raise InvalidArgumentError("query [B, H, D], key_cache [B, Hk, S, D] and value_cache [B, Hk, S, D] are required")
+    if h < 1 or kv_heads < 1 or h % kv_heads:
+        raise InvalidArgumentError(f"the number of query heads ({h}) must be a multiple of the number of key heads ({kv_heads})")
+    if not 1 <= dim <= 256:
+        raise InvalidArgumentError(f"head dimension {dim} is not supported (1 to 256)")
+    _check_side("lengths", lengths, (b,), torch.int32, query)
+    d = _score_options(query, h, scale, softcap, alibi_slopes)
+    d.batch, d.heads, d.kv_heads, d.seq_q, d.seq_k = b, h, kv_heads, 1, sk
+    if prefix_key is not None:
+        _check_same("prefix_key", prefix_key, query)
+        _check_same("prefix_value", prefix_value, query)
+        if prefix_key.dim() != 3 or tuple(prefix_key.shape) != (kv_heads, prefix_key.shape[1], dim) or prefix_value.shape != prefix_key.shape:
+            raise InvalidArgumentError(f"prefix_key and prefix_value must have shape [{kv_heads}, prefix, {dim}]")
+    _require_available()
+    if not query.is_cuda:
+        raise TypeError("query and the caches must be CUDA tensors")
+    query, key_cache, value_cache = _score_operand(query), _score_operand(key_cache), _score_operand(value_cache)
+    if prefix_key is not None and prefix_key.shape[1] > 0:
+        prefix_key, prefix_value = _score_operand(prefix_key), _score_operand(prefix_value)
+        d.prefix_k, d.prefix_v, d.prefix_len = prefix_key.data_ptr(), prefix_value.data_ptr(), prefix_key.shape[1]
+        _set_strides(d, "prefix_k_stride", prefix_key, 2)
+        _set_strides(d, "prefix_v_stride", prefix_value, 2)
+    out = _score_out(out, query)
+    d.q, d.k, d.v, d.out = query.data_ptr(), key_cache.data_ptr() or None, value_cache.data_ptr() or None, out.data_ptr()
+    d.q_stride[:2], d.out_stride[:2] = query.stride()[:2], out.stride()[:2]
+    _set_strides(d, "k_stride", key_cache)
+    _set_strides(d, "v_stride", value_cache)
+    d.key_lengths = lengths.data_ptr() or None
+    lse = None
+    if return_lse:
+        lse = torch.empty((b, h), dtype=torch.float32, device=query.device)
+        d.lse = lse.data_ptr() or None
+    need = int(_b.load_library().sm120_score_attention_decode_workspace_bytes(ctypes.byref(d)))
+    ws = None
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=query.device)      # for this call alone, as in score_attention_grad
+        d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    _score_launch("sm120_launch_score_attention_decode", what, d, query.device)
+    return (out, lse) if return_lse else out
+
+
+def score_attention_decode(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, lengths: torch.Tensor, *,
+                           scale: Optional[float] = None, softcap: Optional[float] = None, alibi_slopes: Optional[torch.Tensor] = None,
+                           return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """The next-token form of ``score_attention`` (``sm120_launch_score_attention_decode``): query [B, H, D], one token
+    per request, over caches [B, Hk, S, D] of which request b has filled the first lengths[b] rows
+    (int32 [B] on the device, clamped to 0 .. S), its own key and value included: the query stands at position
+    lengths[b] - 1.  Cache rows behind that are not read.  A request of length 0 gets zeros.  Same ``scale``,
+    ``softcap`` and ``alibi_slopes``; any cache strides with a contiguous head dimension.  ``return_lse`` adds the
+    float32 [B, H] logarithm of the softmax denominators."""
+    return _score_token("score_attention_decode", query, None, None, key_cache, value_cache, lengths, scale, softcap, alibi_slopes, return_lse, out)
+
+
+def shared_prefix_attention(query: torch.Tensor, prefix_key: torch.Tensor, prefix_value: torch.Tensor, key_cache: torch.Tensor,
+                            value_cache: torch.Tensor, lengths: torch.Tensor, *, scale: Optional[float] = None, softcap: Optional[float] = None,
+                            alibi_slopes: Optional[torch.Tensor] = None, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """``score_attention_decode`` for requests that begin with the same tokens: the keys of request b are
+    [prefix_key | key_cache[b, :, :lengths[b]]] with prefix_key and prefix_value [Hk, P, D], so its query stands at
+    position P + lengths[b] - 1 (a request may have no rows of its own yet).  The prefix is read once per key head
+    for the whole batch, whose queries go through it as the rows of one product; both parts are joined by their
+    softmax denominators."""
+    return _score_token("shared_prefix_attention", query, prefix_key, prefix_value, key_cache, value_cache, lengths, scale, softcap,
+                        alibi_slopes, return_lse, out)
+
+
 class _DenseFunction(torch.autograd.Function):
     """y = relu?(x @ kernel + bias) with this library's kernels in both directions:
     the fused GEMM forward, SM120MatMulGradA / GradB
@@ -1032,6 +1342,11 @@ __all__ = [
     "softmax",
     "scaled_dot_product_attention",
     "flash_attention",
+    "score_attention",
+    "score_attention_grad",
+    "score_attention_trainable",
+    "score_attention_decode",
+    "shared_prefix_attention",
     "quantize_fp8",
     "quantize_fp8_into",
     "SM120Profiler",

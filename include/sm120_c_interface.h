@@ -385,6 +385,105 @@ cudaError_t sm120_launch_attention_ex(
     cudaStream_t stream);
 
 /*
+ * Attention with modified scores, for language models: the forms that
+ * sm120_launch_attention has no argument for.  No counterpart in the reference,
+ * whose attention (python/sm120_ops.py:315-407) knows a scale, an additive mask
+ * and the causal mask; its layer's gradients come from TensorFlow.
+ *
+ * For query row i of entry b and head h, key j, position pos = i + seq_k - seq_q
+ * (queries are aligned to the end of the keys):
+ *   x = scale * <q_i, k_j>
+ *   y = softcap * tanh(x / softcap)           when softcap > 0, else x
+ *   z = y - alibi_slopes[h] * |pos - j|       when alibi_slopes is given, else y
+ *   out_i = sum_j softmax_j(z) v_j            over the keys the row sees
+ *   lse_i = log(sum_j exp(z_j))
+ * A row sees a contiguous range of keys, the intersection of
+ *   causal           j <= pos
+ *   prefix_lengths   with causal: j <= pos or j < prefix_lengths[b]
+ *   document_offsets [batch][num_documents + 1] ascending key positions; a query and
+ *                    a key see each other when both lie in the same
+ *                    [offsets[d], offsets[d+1]); a position before the first or at
+ *                    or behind the last offset sees nothing.  Values outside
+ *                    [0, seq_k] are clamped; unordered ones give an unspecified
+ *                    mask, never an access outside the tensors.
+ * (prefix_lengths and document_offsets are not combined.)  A row that sees no key
+ * has out = 0, lse = -inf and gradients of 0.  Keys that no row of the entry sees
+ * because no document holds them may have any content, NaN included.
+ *
+ * heads is a multiple of kv_heads: query head h reads key/value head
+ * h / (heads / kv_heads).  Tensors are addressed with element strides for entry,
+ * head and row; the head dimension is contiguous and at most 256.  FLOAT16 and
+ * BFLOAT16 with head_dim a multiple of 8 up to 128, 16-byte aligned bases and
+ * strides (and a group of at most 128 heads in the prefix form) run on the tensor
+ * cores; everything else, FLOAT32 included, runs on a plain FFMA kernel.
+ * Statistics and sums are fp32; the tensor-core kernels round the probabilities
+ * (and their gradients) to the inputs' type between the two products.
+ */
+typedef struct SM120ScoreAttentionDesc {
+    uint32_t struct_size;      /* sizeof(SM120ScoreAttentionDesc); checked */
+    int32_t  dtype;            /* SM120DataType of every tensor but lse, alibi_slopes and the integers */
+    int32_t  causal;
+    int32_t  num_documents;    /* 0, or document_offsets has num_documents + 1 entries per batch entry */
+    int64_t  batch, heads, kv_heads, seq_q, seq_k, head_dim;
+    float    scale, softcap;   /* softcap 0 = scores are not capped */
+    const void* q;             /* [batch, heads, seq_q, head_dim] */
+    const void* k;             /* [batch, kv_heads, seq_k, head_dim] */
+    const void* v;
+    void*       out;           /* like q; read by the gradient launch */
+    float*      lse;           /* dense [batch, heads, seq_q], or null (forward); read by the gradient launch */
+    const float*   alibi_slopes;      /* [heads] or null */
+    const int32_t* document_offsets;  /* dense, or null */
+    const int32_t* prefix_lengths;    /* [batch] or null */
+    int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];      /* elements between entries, heads, rows */
+    /* gradient launch */
+    const void* grad_out;
+    void *grad_q, *grad_k, *grad_v;
+    int64_t grad_out_stride[3], grad_q_stride[3], grad_k_stride[3], grad_v_stride[3];
+    /* single-token launch */
+    const int32_t* key_lengths;       /* [batch]: valid rows of k and v per entry, clamped to [0, seq_k] */
+    const void* prefix_k;             /* [kv_heads, prefix_len, head_dim], shared by every entry, or null */
+    const void* prefix_v;
+    int64_t prefix_len;
+    int64_t prefix_k_stride[2], prefix_v_stride[2];                    /* elements between heads, rows */
+    void*    workspace;        /* device scratch owned by the caller, 16-byte aligned */
+    uint64_t workspace_bytes;
+    cudaStream_t stream;
+} SM120ScoreAttentionDesc;
+
+/* Fills *desc with defaults: struct_size, batch = heads = kv_heads = 1, scale = 1, all else 0. */
+void sm120_score_attention_desc_init(SM120ScoreAttentionDesc* desc);
+
+/* Forward: reads q, k, v and writes out and, when given, lse.  Needs no workspace. */
+cudaError_t sm120_launch_score_attention(const SM120ScoreAttentionDesc* desc);
+
+/*
+ * Gradients of the forward launch with the same descriptor: reads q, k, v, out, lse and
+ * grad_out, writes grad_q, grad_k and grad_v (summed over the query heads that
+ * share a key/value head).  With P = exp(z - lse), dP = grad_out V^T and
+ * D_i = <grad_out_i, out_i>:
+ *   dz = P (dP - D),  dx = dz (1 - tanh^2(x / softcap)),
+ *   grad_q = scale dx K,  grad_k = scale dx^T Q,  grad_v = P^T grad_out.
+ * Sums run in a fixed order (no atomics): results are bitwise reproducible.  The
+ * workspace has sm120_score_attention_grad_workspace_bytes(desc) bytes at least;
+ * its contents before the call do not matter.
+ */
+size_t sm120_score_attention_grad_workspace_bytes(const SM120ScoreAttentionDesc* desc);
+cudaError_t sm120_launch_score_attention_grad(const SM120ScoreAttentionDesc* desc);
+
+/*
+ * Next-token form: seq_q = 1 query per entry at the last position of the entry's
+ * keys, [prefix_k | k[b, :, :key_lengths[b]]]: the prefix (if any) is shared by the
+ * batch, and read once per key/value head for all of it.  z uses
+ * pos = prefix_len + key_lengths[b] - 1, which is every key's bound; causal,
+ * document_offsets and prefix_lengths must be off.  Rows of k and v at or behind
+ * key_lengths[b] are not read and may have any content.  An entry without keys has out = 0, lse = -inf.
+ * The keys are split over the GPU and the parts joined in a fixed order; the
+ * workspace has sm120_score_attention_decode_workspace_bytes(desc) bytes at least.
+ */
+size_t sm120_score_attention_decode_workspace_bytes(const SM120ScoreAttentionDesc* desc);
+cudaError_t sm120_launch_score_attention_decode(const SM120ScoreAttentionDesc* desc);
+
+/*
  * Bias gradient of the Dense layer: grad_bias[n] = sum over m of grad_c[m, n] for a
  * row-major [M, N] matrix with row pitch ld (elements; 0 = N), accumulated in fp32
  * in a fixed order (bitwise reproducible; no atomics, no scratch) and written as
