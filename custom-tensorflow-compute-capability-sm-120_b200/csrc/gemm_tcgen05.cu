@@ -139,6 +139,63 @@ bool tc_encode_3d(CUtensorMap* map, const void* ptr, int dtype, int64_t inner, i
     return encode_3d(map, ptr, dtype, inner, outer, nbatch, pitch, bstride, box_inner, box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// 4-D maps (score-modified attention): dims[0] contiguous elements, the other three extents `strides` elements apart.
+// A thread-local table of their own, as above.
+struct MapKey4 {
+    uint64_t ptr, dims[4], stride_bytes[3];
+    uint32_t box[4], dtype, pad;
+};
+static_assert(sizeof(MapKey4) == 88, "MapKey4 must have no padding: it is compared with memcmp");
+struct MapSlot4 {
+    MapKey4 key;
+    CUtensorMap map;
+    bool used;
+};
+static thread_local MapSlot4 t_map4_cache[MAP_CACHE_SLOTS];
+
+bool tc_encode_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&dims)[4], const int64_t (&strides)[3], const int (&box)[4]) {
+    const uint64_t es = static_cast<uint64_t>(dtype_size(dtype));
+    MapKey4 key{};
+    key.ptr = reinterpret_cast<uint64_t>(ptr);
+    key.dtype = static_cast<uint32_t>(dtype);
+    for (int i = 0; i < 4; ++i) {
+        key.dims[i] = static_cast<uint64_t>(dims[i]);
+        key.box[i] = static_cast<uint32_t>(box[i]);
+    }
+    // a stride that no second element uses may be anything in the caller's tensor; the encoder wants a valid one
+    for (int i = 0; i < 3; ++i) key.stride_bytes[i] = dims[i + 1] > 1 ? static_cast<uint64_t>(strides[i]) * es : 16;
+    uint64_t h = 0x9E3779B97F4A7C15ull;
+    for (size_t i = 0; i < sizeof(key) / 8; ++i) {
+        uint64_t w;
+        memcpy(&w, reinterpret_cast<const char*>(&key) + 8 * i, 8);
+        h = (h ^ w) * 0xFF51AFD7ED558CCDull;
+        h ^= h >> 29;
+    }
+    MapSlot4& slot = t_map4_cache[h & (MAP_CACHE_SLOTS - 1)];
+    if (slot.used && memcmp(&slot.key, &key, sizeof(key)) == 0) {
+        *map = slot.map;
+        g_map_hits.fetch_add(1, std::memory_order_relaxed);
+        return true;
+    }
+    EncodeTiledFn fn = get_encode_fn();
+    if (fn == nullptr) return false;
+    cuuint64_t d[4], st[3];
+    cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 4; ++i) {
+        d[i] = key.dims[i];
+        b[i] = key.box[i];
+    }
+    for (int i = 0; i < 3; ++i) st[i] = key.stride_bytes[i];
+    if (fn(map, tmap_dtype(dtype), 4, const_cast<void*>(ptr), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    g_map_encodes.fetch_add(1, std::memory_order_relaxed);
+    slot.key = key;
+    slot.map = *map;
+    slot.used = true;
+    return true;
+}
+
 // Device address of `device`'s status words (looked up once per device, with that device current).
 unsigned int* tc_status_address(int device) {
     static std::atomic<unsigned int*> status_addr[64];

@@ -1311,6 +1311,8 @@ sm120_gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
 bool tc_encode_3d(CUtensorMap* map, const void* ptr, int dtype, int64_t inner, int64_t outer, int64_t nbatch, int64_t pitch,
                   int64_t bstride, uint32_t box_inner, uint32_t box_outer);
 unsigned int* tc_status_address(int device);
+// 4-D map over a strided [dims[3], dims[2], dims[1], dims[0]] tensor, 128-byte swizzle
+bool tc_encode_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&dims)[4], const int64_t (&strides)[3], const int (&box)[4]);
 
 // ---------------------------------------------------------------------------
 // Host-side launch of one kernel variant.  Each variant is instantiated in its

@@ -99,8 +99,9 @@ cudaError_t sm120_launch_score_attention(const SM120ScoreAttentionDesc* desc) {
     int device = 0, sms = 0;
     e = current_device(&device, &sms);
     if (e != cudaSuccess) return e;
-    e = sa_simt_forward(p, desc->stream);
-    if (e == cudaSuccess) note_launches("score_attention_simt", 1);
+    const bool tc = sa_tc_forward_supported(p);
+    e = tc ? sa_tc_forward(p, device, desc->stream) : sa_simt_forward(p, desc->stream);
+    if (e == cudaSuccess) note_launches(tc ? (p.head_dim > 64 ? "score_attention_tcgen05_d128" : "score_attention_tcgen05_d64") : "score_attention_simt", 1);
     return e;
 }
 

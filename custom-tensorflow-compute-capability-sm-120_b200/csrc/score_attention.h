@@ -72,6 +72,10 @@ cudaError_t sa_simt_forward(const ScoreParams& p, cudaStream_t stream);
 cudaError_t sa_simt_grad(const ScoreParams& p, cudaStream_t stream);
 cudaError_t sa_simt_decode(const ScoreParams& p, cudaStream_t stream);
 
+// Tensor-core forward (score_attention_tcgen05.cuh): 16-bit types, head dimension a multiple of 8 up to 128, operands that TMA can address.
+bool sa_tc_forward_supported(const ScoreParams& p);
+cudaError_t sa_tc_forward(const ScoreParams& p, int device, cudaStream_t stream);
+
 // Launcher state shared with launcher.cu: the current device (compute capability 10.x), the wait limit, and the
 // bookkeeping behind sm120_get_launch_count / sm120_get_last_kernel_name.
 cudaError_t current_device(int* device, int* sm_count);
