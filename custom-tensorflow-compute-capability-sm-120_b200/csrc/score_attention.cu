@@ -11,8 +11,6 @@ namespace {
 constexpr int64_t INT31 = (1ll << 31) - 1;
 constexpr int64_t MAX_ROWS = 1ll << 32;       // rows of one launch (four to a block of the plain kernels)
 
-size_t align16(size_t n) { return (n + 15) & ~static_cast<size_t>(15); }
-
 enum class Form { FORWARD, GRADIENT, TOKEN };
 
 // Checks what can be checked without a device and fills `p`.  *empty: nothing to compute.
@@ -31,7 +29,7 @@ cudaError_t resolve(const SM120ScoreAttentionDesc* d, Form form, ScoreParams* p,
     const bool token = form == Form::TOKEN;
     if (token && (d->seq_q != 1 || d->causal || d->num_documents > 0 || d->prefix_lengths != nullptr)) return cudaErrorInvalidValue;
     if (!token && (d->key_lengths != nullptr || d->prefix_len != 0)) return cudaErrorInvalidValue;
-    if (d->batch * d->heads * (d->seq_q + SA_ROW_PAD) > MAX_ROWS || d->batch * d->kv_heads * d->seq_k > MAX_ROWS) return cudaErrorInvalidValue;
+    if (d->batch * d->heads * (d->seq_q + SA_GRAD_TILE + SA_ROW_PAD) > MAX_ROWS || d->batch * d->kv_heads * d->seq_k > MAX_ROWS) return cudaErrorInvalidValue;
     for (int a = 0; a < 3; ++a) {
         if (d->q_stride[a] < 0 || d->k_stride[a] < 0 || d->v_stride[a] < 0 || d->out_stride[a] < 0) return cudaErrorInvalidValue;
         if (form == Form::GRADIENT && (d->grad_out_stride[a] < 0 || d->grad_q_stride[a] < 0 || d->grad_k_stride[a] < 0 || d->grad_v_stride[a] < 0))
@@ -51,7 +49,7 @@ cudaError_t resolve(const SM120ScoreAttentionDesc* d, Form form, ScoreParams* p,
     p->batch = static_cast<int>(d->batch); p->heads = static_cast<int>(d->heads); p->kv_heads = static_cast<int>(d->kv_heads);
     p->group = p->heads / p->kv_heads;
     p->seq_q = static_cast<int>(d->seq_q); p->seq_k = static_cast<int>(d->seq_k); p->head_dim = static_cast<int>(d->head_dim);
-    p->seq_q_pad = (p->seq_q + SA_ROW_PAD - 1) / SA_ROW_PAD * SA_ROW_PAD;
+    p->seq_q_pad = (p->seq_q + SA_GRAD_TILE + SA_ROW_PAD - 1) / SA_ROW_PAD * SA_ROW_PAD;
     p->dtype = d->dtype; p->causal = d->causal != 0; p->num_documents = d->num_documents;
     p->scale = d->scale; p->softcap = d->softcap;
     p->slopes = d->alibi_slopes; p->document_offsets = d->document_offsets; p->prefix_lengths = d->prefix_lengths;
@@ -69,8 +67,10 @@ cudaError_t resolve(const SM120ScoreAttentionDesc* d, Form form, ScoreParams* p,
     return cudaSuccess;
 }
 
-size_t stats_bytes(const ScoreParams& p) { return align16(static_cast<size_t>(p.batch) * p.heads * p.seq_q_pad * sizeof(float2)); }
-size_t ranges_bytes(const ScoreParams& p) { return align16(static_cast<size_t>(p.batch) * p.seq_q_pad * sizeof(int2)); }
+// the three arrays of the gradient workspace; seq_q_pad keeps each a multiple of 16 bytes
+size_t stats_bytes(const ScoreParams& p) { return static_cast<size_t>(p.batch) * p.heads * p.seq_q_pad * sizeof(float); }
+size_t ranges_bytes(const ScoreParams& p) { return static_cast<size_t>(p.batch) * p.seq_q_pad * sizeof(int2); }
+size_t grad_workspace(const ScoreParams& p) { return 2 * stats_bytes(p) + ranges_bytes(p); }
 
 bool workspace_ok(const SM120ScoreAttentionDesc* d, size_t need) {
     return need == 0 || (d->workspace != nullptr && (reinterpret_cast<uintptr_t>(d->workspace) & 15u) == 0 && d->workspace_bytes >= need);
@@ -109,7 +109,7 @@ size_t sm120_score_attention_grad_workspace_bytes(const SM120ScoreAttentionDesc*
     ScoreParams p{};
     bool empty = false;
     if (resolve(desc, Form::GRADIENT, &p, &empty) != cudaSuccess || empty) return 0;
-    return stats_bytes(p) + ranges_bytes(p);
+    return grad_workspace(p);
 }
 
 cudaError_t sm120_launch_score_attention_grad(const SM120ScoreAttentionDesc* desc) {
@@ -117,16 +117,19 @@ cudaError_t sm120_launch_score_attention_grad(const SM120ScoreAttentionDesc* des
     bool empty = false;
     cudaError_t e = resolve(desc, Form::GRADIENT, &p, &empty);
     if (e != cudaSuccess || empty) return e;
-    if (!workspace_ok(desc, stats_bytes(p) + ranges_bytes(p))) return cudaErrorInvalidValue;
+    if (!workspace_ok(desc, grad_workspace(p))) return cudaErrorInvalidValue;
     int device = 0, sms = 0;
     e = current_device(&device, &sms);
     if (e != cudaSuccess) return e;
-    p.stats = static_cast<float2*>(desc->workspace);
-    p.ranges = reinterpret_cast<int2*>(static_cast<char*>(desc->workspace) + stats_bytes(p));
+    p.neg_lse = static_cast<float*>(desc->workspace);
+    p.neg_delta = p.neg_lse + stats_bytes(p) / sizeof(float);
+    p.ranges = reinterpret_cast<int2*>(p.neg_delta + stats_bytes(p) / sizeof(float));
     e = sa_grad_prepare_launch(p, desc->stream);
     if (e != cudaSuccess) return e;
-    e = sa_simt_grad(p, desc->stream);
-    if (e == cudaSuccess) note_launches("score_attention_grad_simt", 3);
+    const bool tc = sa_tc_grad_supported(p);
+    e = tc ? sa_tc_grad(p, device, desc->stream) : sa_simt_grad(p, desc->stream);
+    if (e == cudaSuccess)
+        note_launches(tc ? (p.head_dim > 64 ? "score_attention_grad_tcgen05_d128" : "score_attention_grad_tcgen05_d64") : "score_attention_grad_simt", 3);
     return e;
 }
 

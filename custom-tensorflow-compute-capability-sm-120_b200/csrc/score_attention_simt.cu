@@ -121,7 +121,7 @@ sa_simt_forward_kernel(const ScoreParams p) {
     if (p.lse != nullptr && lane == 0) p.lse[row] = l == 0.0f ? -CUDART_INF_F : m + logf(l);
 }
 
-// stats and ranges of one row per warp, rows behind seq_q included.  One pass over out and grad_out.
+// neg_lse, neg_delta and ranges of one row per warp, rows behind seq_q included.  One pass over out and grad_out.
 template <typename T>
 __global__ void __launch_bounds__(SIMT_WARPS * 32)
 sa_grad_prepare_kernel(const ScoreParams p) {
@@ -131,7 +131,7 @@ sa_grad_prepare_kernel(const ScoreParams p) {
     const int i = static_cast<int>(row % p.seq_q_pad);
     const int64_t bh = row / p.seq_q_pad;
     const int h = static_cast<int>(bh % p.heads), b = static_cast<int>(bh / p.heads);
-    float2 st = make_float2(CUDART_INF_F, 0.0f);
+    float neg_lse = -CUDART_INF_F, neg_delta = 0.0f;
     int2 range = make_int2(0, 0);
     if (i < p.seq_q) {
         const T* o = static_cast<const T*>(p.out) + b * p.o_st[0] + h * p.o_st[1] + i * p.o_st[2];
@@ -141,20 +141,24 @@ sa_grad_prepare_kernel(const ScoreParams p) {
         d = warp_sum(d);
         sa_row_range(p, b, i, range.x, range.y);
         const float lse = p.lse[bh * p.seq_q + i];
-        if (range.x < range.y && lse != -CUDART_INF_F) st = make_float2(lse * SA_LOG2E, d);
+        if (range.x < range.y && lse != -CUDART_INF_F) {
+            neg_lse = -lse * SA_LOG2E;
+            neg_delta = -d;
+        }
     }
     if (lane == 0) {
-        p.stats[row] = st;
+        p.neg_lse[row] = neg_lse;
+        p.neg_delta[row] = neg_delta;
         if (h == 0) p.ranges[static_cast<int64_t>(b) * p.seq_q_pad + i] = range;
     }
 }
 
 // dx (the gradient of the scaled product) and P of one score
-__device__ __forceinline__ float score_grad(float dot, float dp, const float2& st, const ScoreParams& p, float slope, int distance, float& prob) {
+__device__ __forceinline__ float score_grad(float dot, float dp, float neg_lse, float neg_delta, const ScoreParams& p, float slope, int distance, float& prob) {
     float curve;
     const float z = modified_score(dot, p, slope, distance, curve);
-    prob = exp2f(z * SA_LOG2E - st.x);
-    return prob * (dp - st.y) * (1.0f - curve * curve);
+    prob = exp2f(z * SA_LOG2E + neg_lse);
+    return prob * (dp + neg_delta) * (1.0f - curve * curve);
 }
 
 template <typename T>
@@ -172,7 +176,7 @@ sa_simt_grad_q_kernel(const ScoreParams p) {
     const T* k = static_cast<const T*>(p.k) + b * p.k_st[0] + kvh * p.k_st[1];
     const T* v = static_cast<const T*>(p.v) + b * p.v_st[0] + kvh * p.v_st[1];
     const int2 range = p.ranges[static_cast<int64_t>(b) * p.seq_q_pad + i];
-    const float2 st = p.stats[bh * p.seq_q_pad + i];
+    const float neg_lse = p.neg_lse[bh * p.seq_q_pad + i], neg_delta = p.neg_delta[bh * p.seq_q_pad + i];
     const int pos = i + p.seq_k - p.seq_q;
     for (int c = lane; c < p.head_dim; c += 32) {
         q_s[warp][c] = to_f(q[c]);
@@ -183,13 +187,13 @@ sa_simt_grad_q_kernel(const ScoreParams p) {
     float acc[SIMT_COLS];
 #pragma unroll
     for (int t = 0; t < SIMT_COLS; ++t) acc[t] = 0.0f;
-    if (st.x != CUDART_INF_F) {
+    if (neg_lse != -CUDART_INF_F) {
         for (int j0 = range.x; j0 < range.y; j0 += 32) {
             const int j = j0 + lane;
             float dx = 0.0f, prob;
             if (j < range.y)
-                dx = score_grad(dot_row(q_s[warp], k + j * p.k_st[2], p.head_dim), dot_row(g_s[warp], v + j * p.v_st[2], p.head_dim), st, p, slope,
-                                abs(pos - j), prob);
+                dx = score_grad(dot_row(q_s[warp], k + j * p.k_st[2], p.head_dim), dot_row(g_s[warp], v + j * p.v_st[2], p.head_dim), neg_lse,
+                                neg_delta, p, slope, abs(pos - j), prob);
             const int n = min(32, range.y - j0);
             for (int s = 0; s < n; ++s) {
                 const float ws = __shfl_sync(0xFFFFFFFFu, dx, s);
@@ -230,7 +234,7 @@ sa_simt_grad_kv_kernel(const ScoreParams p) {
     for (int h = kvh * p.group; h < (kvh + 1) * p.group; ++h) {
         const T* q = static_cast<const T*>(p.q) + b * p.q_st[0] + h * p.q_st[1];
         const T* g = static_cast<const T*>(p.grad_out) + b * p.go_st[0] + h * p.go_st[1];
-        const float2* stats = p.stats + (static_cast<int64_t>(b) * p.heads + h) * p.seq_q_pad;
+        const int64_t stat_row = (static_cast<int64_t>(b) * p.heads + h) * p.seq_q_pad;
         const float slope = p.slopes != nullptr ? p.slopes[h] : 0.0f;
         for (int i0 = 0; i0 < p.seq_q; i0 += 32) {
             const int i = i0 + lane;
@@ -238,11 +242,11 @@ sa_simt_grad_kv_kernel(const ScoreParams p) {
             float dx = 0.0f, prob = 0.0f;
             if (i < p.seq_q) {
                 const int2 range = ranges[i];
-                const float2 st = stats[i];
-                sees = range.x <= j && j < range.y && st.x != CUDART_INF_F;
+                const float neg_lse = p.neg_lse[stat_row + i];
+                sees = range.x <= j && j < range.y && neg_lse != -CUDART_INF_F;
                 if (sees)
-                    dx = score_grad(dot_row(k_s[warp], q + i * p.q_st[2], p.head_dim), dot_row(v_s[warp], g + i * p.go_st[2], p.head_dim), st, p,
-                                    slope, abs(i + p.seq_k - p.seq_q - j), prob);
+                    dx = score_grad(dot_row(k_s[warp], q + i * p.q_st[2], p.head_dim), dot_row(v_s[warp], g + i * p.go_st[2], p.head_dim), neg_lse,
+                                    p.neg_delta[stat_row + i], p, slope, abs(i + p.seq_k - p.seq_q - j), prob);
             }
             unsigned left = __ballot_sync(0xFFFFFFFFu, sees);
             while (left != 0u) {

@@ -58,10 +58,6 @@ struct SaCfg {
     static_assert(SMEM <= 232448, "shared memory budget exceeded");
 };
 
-// Which formula the distance bias of a tile takes: every key at or before every query (or masked), every key at or
-// behind, or key by key
-enum : int { SA_SIDE_BEFORE = 0, SA_SIDE_BEHIND = 1, SA_SIDE_MIXED = 2 };
-
 // The scores of one row against ATT_BN keys: raw products in, log2-unit modified scores out.  `rel` is the first key's
 // position minus the query's.
 template <bool CAP, bool BIAS>
