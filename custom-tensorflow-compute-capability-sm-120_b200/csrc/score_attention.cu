@@ -134,8 +134,11 @@ cudaError_t sm120_launch_score_attention_grad(const SM120ScoreAttentionDesc* des
 }
 
 size_t sm120_score_attention_decode_workspace_bytes(const SM120ScoreAttentionDesc* desc) {
-    (void)desc;
-    return 0;
+    ScoreParams p{};
+    bool empty = false;
+    int device = 0, sms = 0;
+    if (resolve(desc, Form::TOKEN, &p, &empty) != cudaSuccess || empty || current_device(&device, &sms) != cudaSuccess) return 0;
+    return sa_tc_decode_supported(p) ? sa_tc_decode_workspace(p, sms) : 0;
 }
 
 cudaError_t sm120_launch_score_attention_decode(const SM120ScoreAttentionDesc* desc) {
@@ -146,8 +149,15 @@ cudaError_t sm120_launch_score_attention_decode(const SM120ScoreAttentionDesc* d
     int device = 0, sms = 0;
     e = current_device(&device, &sms);
     if (e != cudaSuccess) return e;
-    e = sa_simt_decode(p, desc->stream);
-    if (e == cudaSuccess) note_launches("score_attention_decode_simt", 1);
+    if (!sa_tc_decode_supported(p)) {
+        e = sa_simt_decode(p, desc->stream);
+        if (e == cudaSuccess) note_launches("score_attention_decode_simt", 1);
+        return e;
+    }
+    if (!workspace_ok(desc, sa_tc_decode_workspace(p, sms))) return cudaErrorInvalidValue;
+    int launches = 0;
+    e = sa_tc_decode(p, desc->workspace, device, sms, desc->stream, &launches);
+    if (e == cudaSuccess) note_launches(p.head_dim > 64 ? "score_attention_decode_d128" : "score_attention_decode_d64", launches);
     return e;
 }
 

@@ -106,6 +106,13 @@ cudaError_t sa_tc_forward(const ScoreParams& p, int device, cudaStream_t stream)
 bool sa_tc_grad_supported(const ScoreParams& p);
 cudaError_t sa_tc_grad(const ScoreParams& p, int device, cudaStream_t stream);
 
+// Single-token form for 16-bit types (score_attention_decode.cu): the same limits.
+bool sa_tma_ok(const void* ptr, const int64_t* strides, const int64_t* extents, int count);
+bool sa_tc_types_ok(const ScoreParams& p);
+bool sa_tc_decode_supported(const ScoreParams& p);
+size_t sa_tc_decode_workspace(const ScoreParams& p, int sms);
+cudaError_t sa_tc_decode(const ScoreParams& p, void* workspace, int device, int sms, cudaStream_t stream, int* launches);
+
 // Launcher state shared with launcher.cu: the current device (compute capability 10.x), the wait limit, and the
 // bookkeeping behind sm120_get_launch_count / sm120_get_last_kernel_name.
 cudaError_t current_device(int* device, int* sm_count);

@@ -1,0 +1,455 @@
+// Single-token attention over a cache, and over a prefix that the batch shares (16-bit types, head
+// dimension up to 128).  Bound by HBM: every valid row of K and V is read once, 4 head_dim operations
+// per query head and 4 head_dim bytes.
+//
+// Parts.  The keys of one (entry, key head) are cut into parts so that short batches fill the GPU and ragged ones
+// balance; each part is one block, writes its normalised fp32 rows and their log2 denominators to the workspace, and
+// a second kernel joins a row's parts in ascending order.  A single part writes the result itself.
+//
+// Block.  Four warps, each with its own ring of 16-key tiles (K and V rows by 16-byte cp.async, rows behind the
+// valid ones never touched: zero fill), so no barrier orders the loop: three tiles of 8 KB per warp and two blocks per SM keep
+// ~190 KB of loads in flight per SM, four times what HBM latency asks for.  The query rows that share the keys (the heads of a
+// group; for the prefix, all entries' heads) are the 16 rows of mma.sync.m16n8k16: the products need a tenth of the
+// legacy tensor rate at full HBM speed, and 16 rows are what one token per request offers, so tcgen05's 128-row tiles would
+// be 7/8 padding.  Both operands come from the swizzled tile by ldmatrix; P goes from the first product's accumulators
+// straight into the second's operand.
+//
+// Rounding.  P is split into two 16-bit pieces (P = hi + lo to 2^-17 relative) that both multiply V: the second product is free
+// under the memory time and the result then carries only its own final rounding.
+//
+// The shared prefix, when the batch has many rows, runs as 128-row tiles on the tcgen05 kernel instead (TOKEN variant of
+// score_attention_tcgen05.cuh) and joins here in the same way.
+
+#include <math_constants.h>
+
+#include "attention_common.cuh"
+#include "score_attention.h"
+
+namespace sm120 {
+
+constexpr int DEC_WARPS = 4;
+constexpr int DEC_ROWS = 16;                  // query rows per block (M of the product)
+constexpr int DEC_KEYS = 16;                  // keys per warp tile
+constexpr int DEC_STAGES = 3;
+constexpr int DEC_STEP = DEC_WARPS * DEC_KEYS;     // keys per turn of the block; parts are multiples of it
+
+// One source of keys: rows [0, rows) of it belong to one key head; row tile t holds rows [16 t, 16 t + 16)
+struct DecodeSide {
+    const void *k, *v;
+    int64_t k_st[3], v_st[3];
+    int row_tiles;                            // per (entry, key head) or, for the prefix, per key head
+    int part_keys, parts;
+    int first_part;                           // index of its first part in the workspace
+    int blocks;                               // row_tiles * parts * key heads (* batch)
+};
+
+struct DecodeParams {
+    ScoreParams s;
+    DecodeSide prefix, own;
+    float scale_log2, cap_in, cap_log2;
+    float* part_out;                          // [part][batch][heads][head_dim]
+    float* part_lse;                          // [part][batch][heads], log2 units
+    int direct;                               // one part in all: write the result itself
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    const int bytes = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// {a, b} = hi + lo, both packed in the 16-bit type
+template <bool BF16>
+__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack16(a, b, BF16);
+    float ha, hb;
+    if constexpr (BF16) {
+        ha = __uint_as_float(hi << 16);
+        hb = __uint_as_float(hi & 0xFFFF0000u);
+    } else {
+        const __half2 h = *reinterpret_cast<const __half2*>(&hi);
+        ha = __low2float(h);
+        hb = __high2float(h);
+    }
+    lo = pack16(a - ha, b - hb, BF16);
+}
+
+template <int D, bool BF16, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(DEC_WARPS * 32, 2)
+sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
+    constexpr int CH = D / 8;                            // 16-byte pieces per row
+    constexpr uint32_t TILE = DEC_KEYS * D * 2;          // bytes of one K (or V) tile
+    constexpr int KSTEPS = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const ScoreParams& sp = p.s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // blocks: the prefix's first, then the caches'; parts vary slowest, so the blocks that leave at once (a part behind an entry's
+    // length) do not crowd together at one place of the grid
+    int idx = static_cast<int>(blockIdx.x);
+    const bool common = idx < p.prefix.blocks;
+    if (!common) idx -= p.prefix.blocks;
+    const DecodeSide& side = common ? p.prefix : p.own;
+    const int rt = idx % side.row_tiles;
+    idx /= side.row_tiles;
+    const int kvh = idx % sp.kv_heads;
+    idx /= sp.kv_heads;
+    const int b = common ? 0 : idx % sp.batch;
+    const int part = common ? idx : idx / sp.batch;
+    const int row0 = rt * DEC_ROWS, n_rows = min(DEC_ROWS, (common ? sp.batch * sp.group : sp.group) - row0);
+    const int total = common ? sp.prefix_len : min(max(__ldg(sp.key_lengths + b), 0), sp.seq_k);
+    const int lo = part * side.part_keys, hi = min(total, lo + side.part_keys);
+    if (lo >= hi && !(p.direct && part == 0)) return;    // the join does not read this part
+
+    // query fragments: rows lane / 4 and lane / 4 + 8, columns 2 (lane % 4) + {0, 1, 8, 9} of each K step
+    auto row_entry = [&](int r) { return common ? (row0 + r) / sp.group : b; };
+    auto row_head = [&](int r) { return kvh * sp.group + (common ? (row0 + r) % sp.group : row0 + r); };
+    uint32_t qf[KSTEPS][4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = (lane >> 2) + 8 * half;
+        const bool live = r < n_rows;
+        const uint16_t* q = static_cast<const uint16_t*>(sp.q) + (live ? row_entry(r) * sp.q_st[0] + row_head(r) * sp.q_st[1] : 0);
+#pragma unroll
+        for (int t = 0; t < KSTEPS; ++t)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int col = t * 16 + c * 8 + (lane & 3) * 2;
+                qf[t][c * 2 + half] = live && col < sp.head_dim ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
+            }
+    }
+    float slope[2] = {0.0f, 0.0f}, pos[2] = {0.0f, 0.0f};
+    if constexpr (BIAS) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = min((lane >> 2) + 8 * half, n_rows - 1);
+            slope[half] = __ldg(sp.slopes + row_head(r)) * SA_LOG2E;
+            // keys of the cache follow the prefix: both count from the side's own first key here
+            const int len = min(max(__ldg(sp.key_lengths + row_entry(r)), 0), sp.seq_k);
+            pos[half] = static_cast<float>(len - 1 + (common ? sp.prefix_len : 0));
+        }
+    }
+
+    const uint32_t ring = smem_u32(smem) + warp * (DEC_STAGES * 2 * TILE);
+    const char* kp = reinterpret_cast<const char*>(static_cast<const uint16_t*>(side.k) + b * side.k_st[0] + kvh * side.k_st[1]);
+    const char* vp = reinterpret_cast<const char*>(static_cast<const uint16_t*>(side.v) + b * side.v_st[0] + kvh * side.v_st[1]);
+    const int64_t k_row = side.k_st[2] * 2, v_row = side.v_st[2] * 2;
+    const int n_tiles = hi > lo ? (hi - lo + DEC_KEYS - 1) / DEC_KEYS : 0;          // of the block; warp w takes w, w + 4, ...
+    auto load = [&](int tile, int stage) {
+        const uint32_t dst = ring + stage * (2 * TILE);
+#pragma unroll
+        for (int i = 0; i < DEC_KEYS * CH / 32; ++i) {
+            const int piece = i * 32 + lane, r = piece / CH, c = piece % CH;
+            const int key = lo + tile * DEC_KEYS + r;
+            const bool valid = key < hi && c * 8 < sp.head_dim;
+            const uint32_t at = r * (D * 2) + ((c ^ (r & 7)) << 4);
+            const int64_t src = valid ? key : 0;
+            cp_async16(dst + at, kp + src * k_row + (valid ? c * 16 : 0), valid);
+            cp_async16(dst + TILE + at, vp + src * v_row + (valid ? c * 16 : 0), valid);
+        }
+    };
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < DEC_STAGES - 1; ++st) {
+        if (warp + st * DEC_WARPS < n_tiles) load(warp + st * DEC_WARPS, st);
+        cp_async_commit();
+    }
+    int stage = 0;
+    for (int tile = warp; tile < n_tiles; tile += DEC_WARPS) {
+        {
+            const int ahead = tile + (DEC_STAGES - 1) * DEC_WARPS;
+            const int into = stage == 0 ? DEC_STAGES - 1 : stage - 1;
+            if (ahead < n_tiles) load(ahead, into);
+            cp_async_commit();
+        }
+        cp_async_wait<DEC_STAGES - 1>();
+        __syncwarp();
+        const uint32_t ks = ring + stage * (2 * TILE), vs = ks + TILE;
+        // S = Q K^T: matrices (keys 0-7, 8-15) x (K columns 0-7, 8-15 of the step)
+        float s[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+        const int kr = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int t = 0; t < KSTEPS; ++t) {
+            uint32_t f[4];
+            const int c = t * 2 + ((lane >> 3) & 1);
+            ldmatrix4(ks + kr * (D * 2) + ((c ^ (kr & 7)) << 4), f);
+            mma16<BF16>(s[0], qf[t], f[0], f[1]);
+            mma16<BF16>(s[1], qf[t], f[2], f[3]);
+        }
+        // scores in log2 units; keys behind the part's end count as nothing
+        const int key0 = lo + tile * DEC_KEYS + (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = key0 + n * 8 + (i & 1);
+                float z = s[n][i];
+                if constexpr (CAP) z = fmaf(att_rcp(att_exp2(z * p.cap_in) + 1.0f), -2.0f * p.cap_log2, p.cap_log2);
+                else z *= p.scale_log2;
+                if constexpr (BIAS) z = fmaf(slope[i >> 1], static_cast<float>(key) - pos[i >> 1], z);
+                s[n][i] = key < hi ? z : -CUDART_INF_F;
+            }
+        uint32_t hi_f[4], lo_f[4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float mx = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+            const float m_new = fmaxf(m[half], mx), m_use = m_new == -CUDART_INF_F ? 0.0f : m_new;
+            if (__any_sync(0xFFFFFFFFu, m_new != m[half])) {
+                const float fade = att_exp2(m[half] - m_use);
+                l[half] *= fade;
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) {
+                    o[n][2 * half] *= fade;
+                    o[n][2 * half + 1] *= fade;
+                }
+                m[half] = m_new;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float p0 = att_exp2(s[n][2 * half] - m_use), p1 = att_exp2(s[n][2 * half + 1] - m_use);
+                l[half] += p0 + p1;
+                split16<BF16>(p0, p1, hi_f[n * 2 + half], lo_f[n * 2 + half]);
+            }
+        }
+        // O += P V: V matrices (keys 0-7, 8-15) x (two blocks of 8 columns), transposed on the way
+        const int vr = (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            uint32_t f[4];
+            const int c = n * 2 + (lane >> 4);
+            ldmatrix4_trans(vs + vr * (D * 2) + ((c ^ (vr & 7)) << 4), f);
+            mma16<BF16>(o[2 * n], hi_f, f[0], f[1]);
+            mma16<BF16>(o[2 * n + 1], hi_f, f[2], f[3]);
+            mma16<BF16>(o[2 * n], lo_f, f[0], f[1]);
+            mma16<BF16>(o[2 * n + 1], lo_f, f[2], f[3]);
+        }
+        __syncwarp();                                    // every lane has read the stage that the next turn's load overwrites
+        if (++stage == DEC_STAGES) stage = 0;
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
+        l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
+    }
+    // join the four warps in shared memory (the rings are done): rows of D floats, then {m, l} per warp and row
+    __syncthreads();
+    float* rows = reinterpret_cast<float*>(smem);                                     // [warp][16][D]
+    float2* ml = reinterpret_cast<float2*>(smem + DEC_WARPS * DEC_ROWS * D * 4);      // [warp][16]
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int r = (lane >> 2) + 8 * half;
+        float* dst = rows + (warp * DEC_ROWS + r) * D + (lane & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+        if ((lane & 3) == 0) ml[warp * DEC_ROWS + r] = make_float2(m[half], l[half]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_rows * (D / 4); i += DEC_WARPS * 32) {
+        const int r = i / (D / 4), col = i % (D / 4) * 4;
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, ml[w * DEC_ROWS + r].x);
+        const float base = top == -CUDART_INF_F ? 0.0f : top;
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < DEC_WARPS; ++w) {
+            const float2 x = ml[w * DEC_ROWS + r];
+            const float f = att_exp2(x.x - base);
+            const float4 y = *reinterpret_cast<const float4*>(rows + (w * DEC_ROWS + r) * D + col);
+            sum = fmaf(f, x.y, sum);
+            acc.x = fmaf(f, y.x, acc.x);
+            acc.y = fmaf(f, y.y, acc.y);
+            acc.z = fmaf(f, y.z, acc.z);
+            acc.w = fmaf(f, y.w, acc.w);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float lse = sum == 0.0f ? -CUDART_INF_F : base + log2f(sum);
+        const int e = row_entry(r), h = row_head(r);
+        const int64_t row = static_cast<int64_t>(e) * sp.heads + h;
+        if (p.direct) {
+            if (col < sp.head_dim)
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(sp.out) + e * sp.o_st[0] + h * sp.o_st[1] + col) =
+                    make_uint2(pack16(acc.x * inv, acc.y * inv, BF16), pack16(acc.z * inv, acc.w * inv, BF16));
+            if (col == 0 && sp.lse != nullptr) sp.lse[row] = lse * SA_LN2;
+        } else {
+            const int64_t at = static_cast<int64_t>(side.first_part + part) * sp.batch * sp.heads + row;
+            if (col < sp.head_dim)
+                *reinterpret_cast<float4*>(p.part_out + at * sp.head_dim + col) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            if (col == 0) p.part_lse[at] = lse;
+        }
+    }
+}
+
+// One warp per row: its parts in ascending order, weights 2^(lse - max)
+template <bool BF16>
+__global__ void __launch_bounds__(128)
+sm120_score_decode_join_kernel(const __grid_constant__ DecodeParams p) {
+    const ScoreParams& sp = p.s;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5), all = static_cast<int64_t>(sp.batch) * sp.heads;
+    if (row >= all) return;
+    const int e = static_cast<int>(row / sp.heads), h = static_cast<int>(row % sp.heads);
+    const int len = min(max(__ldg(sp.key_lengths + e), 0), sp.seq_k);
+    // the parts that were written: all of the prefix's, and the cache's up to the entry's length
+    const int own_parts = p.own.parts > 0 ? (len + p.own.part_keys - 1) / p.own.part_keys : 0;
+    const int parts = p.prefix.parts + own_parts;
+    float top = -CUDART_INF_F;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_lse[i * all + row]);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+    const float base = top == -CUDART_INF_F ? 0.0f : top;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    const int col = lane * 4;
+    const bool mine = col < sp.head_dim;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        const float w = att_exp2(p.part_lse[i * all + row] - base);
+        sum += w;
+        if (mine) {
+            const float4 y = *reinterpret_cast<const float4*>(p.part_out + (i * all + row) * sp.head_dim + col);
+            acc.x = fmaf(w, y.x, acc.x);
+            acc.y = fmaf(w, y.y, acc.y);
+            acc.z = fmaf(w, y.z, acc.z);
+            acc.w = fmaf(w, y.w, acc.w);
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (mine)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(sp.out) + e * sp.o_st[0] + h * sp.o_st[1] + col) =
+            make_uint2(pack16(acc.x * inv, acc.y * inv, BF16), pack16(acc.z * inv, acc.w * inv, BF16));
+    if (lane == 0 && sp.lse != nullptr) sp.lse[row] = sum == 0.0f ? -CUDART_INF_F : (base + log2f(sum)) * SA_LN2;
+}
+
+// How a call is cut.  A part is at least one turn of a block (64 keys) and at most 1024 keys: long caches of ragged length then
+// balance by themselves, and the workspace stays below 2 / 1024 of the cache's traffic per query row.
+struct DecodePlan {
+    DecodeParams p;
+    int64_t parts;
+};
+
+static bool plan_side(DecodeSide& s, int64_t keys, int64_t row_tiles, int64_t heads_and_entries, int64_t fill) {
+    s.row_tiles = static_cast<int>(row_tiles);
+    s.parts = 0;
+    s.blocks = 0;
+    s.part_keys = DEC_STEP;
+    if (keys == 0) return true;
+    const int64_t base = row_tiles * heads_and_entries;
+    int64_t parts = fill > base ? fill / base : 1;                              // parts that fill the GPU
+    int64_t part = (keys + parts - 1) / parts;
+    part = (part + DEC_STEP - 1) / DEC_STEP * DEC_STEP;
+    if (part > 1024) part = 1024;
+    parts = (keys + part - 1) / part;
+    if (parts * base > (1ll << 30)) return false;
+    s.part_keys = static_cast<int>(part);
+    s.parts = static_cast<int>(parts);
+    s.blocks = static_cast<int>(parts * base);
+    return true;
+}
+
+static bool make_plan(const ScoreParams& p, int sms, DecodePlan* plan) {
+    DecodeParams& dp = plan->p;
+    dp = DecodeParams{};
+    dp.s = p;
+    dp.scale_log2 = p.scale * SA_LOG2E;
+    dp.cap_in = p.softcap > 0.0f ? 2.0f * SA_LOG2E * p.scale / p.softcap : 0.0f;
+    dp.cap_log2 = p.softcap * SA_LOG2E;
+    const int64_t fill = 2ll * sms;                                             // two blocks per SM
+    const int64_t rows = static_cast<int64_t>(p.batch) * p.group;
+    if (!plan_side(dp.prefix, p.prefix_len, (rows + DEC_ROWS - 1) / DEC_ROWS, p.kv_heads, fill)) return false;
+    if (!plan_side(dp.own, p.seq_k, (p.group + DEC_ROWS - 1) / DEC_ROWS, static_cast<int64_t>(p.kv_heads) * p.batch, fill)) return false;
+    dp.prefix.k = p.prefix_k; dp.prefix.v = p.prefix_v;
+    dp.prefix.k_st[1] = p.pk_st[0]; dp.prefix.k_st[2] = p.pk_st[1];
+    dp.prefix.v_st[1] = p.pv_st[0]; dp.prefix.v_st[2] = p.pv_st[1];
+    dp.own.k = p.k; dp.own.v = p.v;
+    for (int a = 0; a < 3; ++a) {
+        dp.own.k_st[a] = p.k_st[a];
+        dp.own.v_st[a] = p.v_st[a];
+    }
+    dp.own.first_part = dp.prefix.parts;
+    plan->parts = static_cast<int64_t>(dp.prefix.parts) + dp.own.parts;
+    dp.direct = plan->parts == 1;
+    return static_cast<int64_t>(dp.prefix.blocks) + dp.own.blocks < (1ll << 31);
+}
+
+bool sa_tc_decode_supported(const ScoreParams& p) {
+    if (!sa_tc_types_ok(p) || (p.seq_k < 1 && p.prefix_len < 1)) return false;
+    const int64_t qe[2] = {p.batch, p.heads}, ke[3] = {p.batch, p.kv_heads, p.seq_k}, pe[2] = {p.kv_heads, p.prefix_len};
+    if (!sa_tma_ok(p.q, p.q_st, qe, 2) || !sa_tma_ok(p.out, p.o_st, qe, 2)) return false;
+    if (p.seq_k > 0 && (!sa_tma_ok(p.k, p.k_st, ke, 3) || !sa_tma_ok(p.v, p.v_st, ke, 3))) return false;
+    return p.prefix_len < 1 || (sa_tma_ok(p.prefix_k, p.pk_st, pe, 2) && sa_tma_ok(p.prefix_v, p.pv_st, pe, 2));
+}
+
+size_t sa_tc_decode_workspace(const ScoreParams& p, int sms) {
+    DecodePlan plan;
+    if (!make_plan(p, sms, &plan) || plan.p.direct) return 0;
+    return static_cast<size_t>(plan.parts) * p.batch * p.heads * (p.head_dim + 1) * sizeof(float);
+}
+
+template <int D, bool BF16>
+static cudaError_t decode_launch(const DecodeParams& dp, int device, cudaStream_t stream) {
+    constexpr int SMEM = DEC_WARPS * DEC_STAGES * 2 * DEC_KEYS * D * 2;
+    static_assert(DEC_WARPS * DEC_ROWS * (D * 4 + 8) <= SMEM, "the join's rows fit the rings");
+    const bool cap = dp.s.softcap > 0.0f, bias = dp.s.slopes != nullptr;
+    auto kern = cap ? (bias ? sm120_score_decode_kernel<D, BF16, true, true> : sm120_score_decode_kernel<D, BF16, true, false>)
+                    : (bias ? sm120_score_decode_kernel<D, BF16, false, true> : sm120_score_decode_kernel<D, BF16, false, false>);
+    static std::atomic<uint64_t> attr_done[4];
+    std::atomic<uint64_t>& done = attr_done[(cap ? 2 : 0) + (bias ? 1 : 0)];
+    const uint64_t bit = 1ull << (device & 63);
+    if ((done.load(std::memory_order_acquire) & bit) == 0) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return e;
+        done.fetch_or(bit, std::memory_order_release);
+    }
+    kern<<<static_cast<unsigned>(dp.prefix.blocks + dp.own.blocks), DEC_WARPS * 32, SMEM, stream>>>(dp);
+    return cudaGetLastError();
+}
+
+cudaError_t sa_tc_decode(const ScoreParams& p, void* workspace, int device, int sms, cudaStream_t stream, int* launches) {
+    DecodePlan plan;
+    if (!make_plan(p, sms, &plan)) return cudaErrorInvalidValue;
+    DecodeParams& dp = plan.p;
+    dp.part_out = static_cast<float*>(workspace);
+    dp.part_lse = dp.part_out + plan.parts * p.batch * p.heads * p.head_dim;
+    const bool bf16 = p.dtype == SM120_DTYPE_BFLOAT16;
+    cudaError_t e = p.head_dim > 64 ? (bf16 ? decode_launch<128, true>(dp, device, stream) : decode_launch<128, false>(dp, device, stream))
+                                    : (bf16 ? decode_launch<64, true>(dp, device, stream) : decode_launch<64, false>(dp, device, stream));
+    *launches = 1;
+    if (e != cudaSuccess || dp.direct) return e;
+    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.heads + 3) / 4);
+    if (bf16) sm120_score_decode_join_kernel<true><<<blocks, 128, 0, stream>>>(dp);
+    else sm120_score_decode_join_kernel<false><<<blocks, 128, 0, stream>>>(dp);
+    *launches = 2;
+    return cudaGetLastError();
+}
+
+}  // namespace sm120
