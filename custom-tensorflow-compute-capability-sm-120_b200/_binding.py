@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import (POINTER, Structure, c_bool, c_char_p, c_float, c_int, c_int32, c_int64, c_uint, c_uint32,
                     c_uint64, c_void_p)
 
@@ -93,6 +94,10 @@ class SM120ScoreAttentionDesc(Structure):
         ("workspace_bytes", c_uint64),
         ("stream", c_void_p),
     ]
+
+
+# the same layout for callers that fill all fields at once: one struct.pack instead of some forty attribute stores (about 10 us of host time)
+SCORE_ATTENTION_PACK = struct.Struct("@Iiii6q2f8P12q4P12q3Pq4qPQP")
 
 
 # name -> (restype, argtypes): every symbol the public header declares

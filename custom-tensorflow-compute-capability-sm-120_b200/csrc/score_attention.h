@@ -102,6 +102,10 @@ cudaError_t sa_simt_decode(const ScoreParams& p, cudaStream_t stream);
 bool sa_tc_forward_supported(const ScoreParams& p);
 cudaError_t sa_tc_forward(const ScoreParams& p, int device, cudaStream_t stream);
 
+// The batch's single-token queries against the shared prefix on the same kernel: row tiles of 128 / group entries, the key tiles cut into
+// `parts` parts of `tiles_per_part`, results in part_out / part_lse (score_attention_decode.cu).
+cudaError_t sa_tc_prefix(const ScoreParams& p, int parts, int tiles_per_part, float* part_out, float* part_lse, int device, cudaStream_t stream);
+
 // Tensor-core gradients (score_attention_grad_tcgen05.cuh), after sa_grad_prepare_launch; the same limits.
 bool sa_tc_grad_supported(const ScoreParams& p);
 cudaError_t sa_tc_grad(const ScoreParams& p, int device, cudaStream_t stream);

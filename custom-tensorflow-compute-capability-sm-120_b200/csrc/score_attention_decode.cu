@@ -31,6 +31,12 @@ constexpr int DEC_WARPS = 4;
 constexpr int DEC_ROWS = 16;                  // query rows per block (M of the product)
 constexpr int DEC_KEYS = 16;                  // keys per warp tile
 constexpr int DEC_STAGES = 3;
+// rows x keys x key heads of the prefix from which it runs on the tcgen05 kernel, whose 128-row tiles start slower but read the keys
+// once per 128 rows instead of 16.  Measured, us (here / tcgen05): head size 128, 8 key heads, 4096 keys: 32 rows 14.2 / 16.4, 64 rows
+// 19.4 / 17.2, 256 rows 50 / 27; 1 key head, 16384 keys: 64 rows 16.5 / 18.7, 256 rows 25 / 21; head size 64 crosses half as far again
+// (8 key heads, 4096 keys: 64 rows 13.6 / 14.6, 128 rows 22.1 / 15.9)
+constexpr int64_t PREFIX_TC_WORK_128 = 2ll << 20, PREFIX_TC_WORK_64 = 3ll << 20;
+constexpr int PREFIX_MAX_PARTS = 64;
 constexpr int DEC_STEP = DEC_WARPS * DEC_KEYS;     // keys per turn of the block; parts are multiples of it
 
 // One source of keys: rows [0, rows) of it belong to one key head; row tile t holds rows [16 t, 16 t + 16)
@@ -50,6 +56,7 @@ struct DecodeParams {
     float* part_out;                          // [part][batch][heads][head_dim]
     float* part_lse;                          // [part][batch][heads], log2 units
     int direct;                               // one part in all: write the result itself
+    int prefix_tiles;                         // the prefix runs on the tcgen05 kernel, this many key tiles per part (0: it runs here)
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -309,14 +316,16 @@ sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
     }
 }
 
-// One warp per row: its parts in ascending order, weights 2^(lse - max)
+// One block per row: warp w sums the parts w, w + 4, ... with weights 2^(lse - max), the four sums are added in order.  A row has up to
+// hundreds of parts when few rows share long keys; four warps and four loads in flight keep that a matter of microseconds.
 template <bool BF16>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(DEC_WARPS * 32)
 sm120_score_decode_join_kernel(const __grid_constant__ DecodeParams p) {
+    __shared__ float4 part[DEC_WARPS][32];
+    __shared__ float part_sum[DEC_WARPS];
     const ScoreParams& sp = p.s;
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5), all = static_cast<int64_t>(sp.batch) * sp.heads;
-    if (row >= all) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = blockIdx.x, all = static_cast<int64_t>(sp.batch) * sp.heads;
     const int e = static_cast<int>(row / sp.heads), h = static_cast<int>(row % sp.heads);
     const int len = min(max(__ldg(sp.key_lengths + e), 0), sp.seq_k);
     // the parts that were written: all of the prefix's, and the cache's up to the entry's length
@@ -332,16 +341,27 @@ sm120_score_decode_join_kernel(const __grid_constant__ DecodeParams p) {
     const int col = lane * 4;
     const bool mine = col < sp.head_dim;
 #pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
+    for (int i = warp; i < parts; i += DEC_WARPS) {
         const float w = att_exp2(p.part_lse[i * all + row] - base);
+        const float4 y = *reinterpret_cast<const float4*>(p.part_out + (i * all + row) * sp.head_dim + (mine ? col : 0));
         sum += w;
-        if (mine) {
-            const float4 y = *reinterpret_cast<const float4*>(p.part_out + (i * all + row) * sp.head_dim + col);
-            acc.x = fmaf(w, y.x, acc.x);
-            acc.y = fmaf(w, y.y, acc.y);
-            acc.z = fmaf(w, y.z, acc.z);
-            acc.w = fmaf(w, y.w, acc.w);
-        }
+        acc.x = fmaf(w, y.x, acc.x);
+        acc.y = fmaf(w, y.y, acc.y);
+        acc.z = fmaf(w, y.z, acc.z);
+        acc.w = fmaf(w, y.w, acc.w);
+    }
+    part[warp][lane] = acc;
+    if (lane == 0) part_sum[warp] = sum;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int w = 1; w < DEC_WARPS; ++w) {
+        const float4 y = part[w][lane];
+        sum += part_sum[w];
+        acc.x += y.x;
+        acc.y += y.y;
+        acc.z += y.z;
+        acc.w += y.w;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (mine)
@@ -385,7 +405,24 @@ static bool make_plan(const ScoreParams& p, int sms, DecodePlan* plan) {
     dp.cap_log2 = p.softcap * SA_LOG2E;
     const int64_t fill = 2ll * sms;                                             // two blocks per SM
     const int64_t rows = static_cast<int64_t>(p.batch) * p.group;
-    if (!plan_side(dp.prefix, p.prefix_len, (rows + DEC_ROWS - 1) / DEC_ROWS, p.kv_heads, fill)) return false;
+    if (rows * p.prefix_len * p.kv_heads >= (p.head_dim > 64 ? PREFIX_TC_WORK_128 : PREFIX_TC_WORK_64) && p.group <= ATT_BM) {
+        // one block per SM: parts that even out the last wave, a block's start and end counted as four key tiles
+        const int64_t tiles = (p.prefix_len + ATT_BN - 1) / ATT_BN, per_tile = ATT_BM / p.group;
+        const int64_t base = (p.batch + per_tile - 1) / per_tile * p.kv_heads;
+        int64_t best = INT64_MAX;
+        for (int64_t parts = 1; parts <= tiles && parts <= PREFIX_MAX_PARTS; ++parts) {
+            const int64_t each = (tiles + parts - 1) / parts, cost = (base * parts + sms - 1) / sms * (each + 4);
+            if (cost < best && (parts - 1) * each < tiles) {
+                best = cost;
+                dp.prefix.parts = static_cast<int>(parts);
+                dp.prefix_tiles = static_cast<int>(each);
+            }
+        }
+        dp.prefix.row_tiles = 1;
+        dp.prefix.part_keys = dp.prefix_tiles * ATT_BN;
+    } else if (!plan_side(dp.prefix, p.prefix_len, (rows + DEC_ROWS - 1) / DEC_ROWS, p.kv_heads, fill)) {
+        return false;
+    }
     if (!plan_side(dp.own, p.seq_k, (p.group + DEC_ROWS - 1) / DEC_ROWS, static_cast<int64_t>(p.kv_heads) * p.batch, fill)) return false;
     dp.prefix.k = p.prefix_k; dp.prefix.v = p.prefix_v;
     dp.prefix.k_st[1] = p.pk_st[0]; dp.prefix.k_st[2] = p.pk_st[1];
@@ -397,8 +434,8 @@ static bool make_plan(const ScoreParams& p, int sms, DecodePlan* plan) {
     }
     dp.own.first_part = dp.prefix.parts;
     plan->parts = static_cast<int64_t>(dp.prefix.parts) + dp.own.parts;
-    dp.direct = plan->parts == 1;
-    return static_cast<int64_t>(dp.prefix.blocks) + dp.own.blocks < (1ll << 31);
+    dp.direct = plan->parts == 1 && dp.prefix_tiles == 0;
+    return static_cast<int64_t>(dp.prefix.blocks) + dp.own.blocks < (1ll << 31) && static_cast<int64_t>(p.batch) * p.heads < (1ll << 31);
 }
 
 bool sa_tc_decode_supported(const ScoreParams& p) {
@@ -441,14 +478,24 @@ cudaError_t sa_tc_decode(const ScoreParams& p, void* workspace, int device, int 
     dp.part_out = static_cast<float*>(workspace);
     dp.part_lse = dp.part_out + plan.parts * p.batch * p.heads * p.head_dim;
     const bool bf16 = p.dtype == SM120_DTYPE_BFLOAT16;
-    cudaError_t e = p.head_dim > 64 ? (bf16 ? decode_launch<128, true>(dp, device, stream) : decode_launch<128, false>(dp, device, stream))
-                                    : (bf16 ? decode_launch<64, true>(dp, device, stream) : decode_launch<64, false>(dp, device, stream));
-    *launches = 1;
-    if (e != cudaSuccess || dp.direct) return e;
-    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.batch) * p.heads + 3) / 4);
-    if (bf16) sm120_score_decode_join_kernel<true><<<blocks, 128, 0, stream>>>(dp);
-    else sm120_score_decode_join_kernel<false><<<blocks, 128, 0, stream>>>(dp);
-    *launches = 2;
+    *launches = 0;
+    cudaError_t e = cudaSuccess;
+    if (dp.prefix_tiles > 0) {
+        e = sa_tc_prefix(p, dp.prefix.parts, dp.prefix_tiles, dp.part_out, dp.part_lse, device, stream);
+        if (e != cudaSuccess) return e;
+        ++*launches;
+    }
+    if (dp.prefix.blocks + dp.own.blocks > 0) {
+        e = p.head_dim > 64 ? (bf16 ? decode_launch<128, true>(dp, device, stream) : decode_launch<128, false>(dp, device, stream))
+                            : (bf16 ? decode_launch<64, true>(dp, device, stream) : decode_launch<64, false>(dp, device, stream));
+        if (e != cudaSuccess) return e;
+        ++*launches;
+    }
+    if (dp.direct) return e;
+    const unsigned rows = static_cast<unsigned>(p.batch) * p.heads;
+    if (bf16) sm120_score_decode_join_kernel<true><<<rows, DEC_WARPS * 32, 0, stream>>>(dp);
+    else sm120_score_decode_join_kernel<false><<<rows, DEC_WARPS * 32, 0, stream>>>(dp);
+    ++*launches;
     return cudaGetLastError();
 }
 

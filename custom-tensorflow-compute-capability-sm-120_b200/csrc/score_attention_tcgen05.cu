@@ -52,6 +52,25 @@ cudaError_t sa_tc_forward(const ScoreParams& p, int device, cudaStream_t stream)
     return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, fp, false, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, fp, false, grid, device, stream);
 }
 
+cudaError_t sa_tc_prefix(const ScoreParams& p, int parts, int tiles_per_part, float* part_out, float* part_lse, int device, cudaStream_t stream) {
+    SaFwdParams fp{};
+    sa_fwd_constants(fp, p, device);
+    if (fp.status == nullptr) return cudaErrorInvalidSymbol;
+    fp.batch_per_tile = ATT_BM / p.group;
+    fp.tiles_per_part = tiles_per_part;
+    fp.part_out = part_out;
+    fp.part_lse = part_lse;
+    CUtensorMap tq, tk, tv;
+    const int64_t d = p.head_dim;
+    // queries as [key head][entry][head of the group]: a box of all the group's heads and batch_per_tile entries is a row tile
+    if (!tc_encode_4d(&tq, p.q, p.dtype, {d, p.group, p.batch, p.kv_heads}, {p.q_st[1], p.q_st[0], p.q_st[1] * p.group}, {64, p.group, fp.batch_per_tile, 1}) ||
+        !tc_encode_4d(&tk, p.prefix_k, p.dtype, {d, p.prefix_len, p.kv_heads, 1}, {p.pk_st[1], p.pk_st[0], 0}, {64, ATT_BN, 1, 1}) ||
+        !tc_encode_4d(&tv, p.prefix_v, p.dtype, {d, p.prefix_len, p.kv_heads, 1}, {p.pv_st[1], p.pv_st[0], 0}, {64, 64, 1, 1}))
+        return cudaErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(p.kv_heads), (p.batch + fp.batch_per_tile - 1) / fp.batch_per_tile, parts);
+    return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, fp, true, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, fp, true, grid, device, stream);
+}
+
 extern template cudaError_t sa_grad_launch_d<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaGradParams&, bool, dim3, int, cudaStream_t);
 extern template cudaError_t sa_grad_launch_d<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaGradParams&, bool, dim3, int, cudaStream_t);
 

@@ -809,14 +809,17 @@ def flash_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Ten
 # attention with modified scores: prompts, gradients, next tokens
 # ---------------------------------------------------------------------------
 _SCORE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+_ZERO3, _ZERO2 = (0, 0, 0), (0, 0)
+# the current stream's handle without building a Stream object (2 us of a call whose kernels may take 5)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _check_same(name: str, t, like: torch.Tensor) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.dtype != like.dtype:
+    if t.dtype is not like.dtype:
         raise ValueError(f"{name} must have the query's dtype {like.dtype}, got {t.dtype}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, the query on {like.device}")
 
 
@@ -824,18 +827,39 @@ def _check_side(name: str, t, shape, dtype: torch.dtype, like: torch.Tensor) -> 
     """A small companion tensor (slopes, offsets, lengths, lse): exact shape and dtype, contiguous, on the query's device."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype is not dtype:
         raise InvalidArgumentError(f"{name} must be a {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{name} is on {t.device}, the query on {like.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _check_query(query, dims: int, what: str) -> None:
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a tensor")
+    if query.dtype not in _SCORE_DTYPES:
+        raise ValueError(f"dtype {query.dtype} is not supported (float32, float16, bfloat16)")
+    if query.dim() != dims:
+        raise ValueError(what)
+
+
+def _check_heads(h: int, kv_heads: int, dim: int) -> None:
+    if h < 1 or kv_heads < 1 or h % kv_heads:
+        raise InvalidArgumentError(f"the number of query heads ({h}) must be a multiple of the number of key heads ({kv_heads})")
+    if not 1 <= dim <= 256:
+        raise InvalidArgumentError(f"head dimension {dim} is not supported (1 to 256)")
 
 
 def _score_operand(t: torch.Tensor) -> torch.Tensor:
     """`t` as the tensor-core kernels can address it: contiguous head dimension, and for 16-bit types 16-byte aligned
     with strides that are multiples of 16 bytes.  Other layouts are copied once."""
     strides = t.stride()
+    bits = t.data_ptr() >> 1 if strides[-1] == 1 else 1
+    for st in strides[:-1]:
+        bits |= st if st else 1
+    if not bits & 7:
+        return t                                       # the usual case: nothing to look at any closer
     if strides[-1] != 1 and t.shape[-1] != 1:
         return t.contiguous()
     if t.dtype != torch.float32 and t.shape[-1] % 8 == 0 and t.shape[-1] <= 128:
@@ -845,85 +869,46 @@ def _score_operand(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _score_options(query: torch.Tensor, heads: int, scale: Optional[float], softcap: Optional[float], alibi_slopes) -> _b.SM120ScoreAttentionDesc:
-    d = _b.new_score_attention_desc()
-    d.dtype = _TORCH_TO_SM120[query.dtype]
-    d.head_dim = query.shape[-1]
-    d.scale = 1.0 / float(query.shape[-1]) ** 0.5 if scale is None else float(scale)
-    if d.scale != d.scale:
+def _score_scalars(dim: int, scale: Optional[float], softcap: Optional[float]):
+    scale = 1.0 / dim ** 0.5 if scale is None else float(scale)
+    if scale != scale:
         raise ValueError("scale must not be NaN")
-    if softcap is not None:
-        if not (0.0 < float(softcap) <= 1e30):
-            raise ValueError(f"softcap must be positive (None switches it off), got {softcap}")
-        d.softcap = float(softcap)
-    if alibi_slopes is not None:
-        _check_side("alibi_slopes", alibi_slopes, (heads,), torch.float32, query)
-        d.alibi_slopes = alibi_slopes.data_ptr()
-    return d
+    if softcap is None:
+        return scale, 0.0
+    if not (0.0 < float(softcap) <= 1e30):
+        raise ValueError(f"softcap must be positive (None switches it off), got {softcap}")
+    return scale, float(softcap)
 
 
-def _set_strides(d, name: str, t: torch.Tensor, count: int = 3) -> None:
-    getattr(d, name)[:] = t.stride()[:count]
+def _score_desc(*fields) -> _b.SM120ScoreAttentionDesc:
+    return _b.SM120ScoreAttentionDesc.from_buffer(bytearray(_b.SCORE_ATTENTION_PACK.pack(_b.SCORE_ATTENTION_PACK.size, *fields)))
 
 
-def _score_sequence_desc(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths):
-    """Checks the arguments of the sequence forms and fills a descriptor but for what is written; returns it with the operands it points to."""
-    if not isinstance(query, torch.Tensor):
-        raise TypeError("query must be a tensor")
-    if query.dtype not in _SCORE_DTYPES:
-        raise ValueError(f"dtype {query.dtype} is not supported (float32, float16, bfloat16)")
-    _check_same("key", key, query)
-    _check_same("value", value, query)
-    if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
-        raise ValueError("query, key and value must be 4-dimensional [batch, heads, seq, head_dim]")
-    b, h, sq, dim = query.shape
-    kv_heads, sk = key.shape[1], key.shape[2]
-    if tuple(key.shape) != (b, kv_heads, sk, dim) or tuple(value.shape) != (b, kv_heads, sk, dim):
-        raise InvalidArgumentError("query [B, H, Sq, D], key [B, Hk, Sk, D] and value [B, Hk, Sk, D] are required")
-    if h < 1 or kv_heads < 1 or h % kv_heads:
-        raise InvalidArgumentError(f"the number of query heads ({h}) must be a multiple of the number of key heads ({kv_heads})")
-    if not 1 <= dim <= 256:
-        raise InvalidArgumentError(f"head dimension {dim} is not supported (1 to 256)")
-    d = _score_options(query, h, scale, softcap, alibi_slopes)
-    d.causal = int(bool(causal_mask))
-    d.batch, d.heads, d.kv_heads, d.seq_q, d.seq_k = b, h, kv_heads, sq, sk
-    if document_offsets is not None:
-        if prefix_lengths is not None:
-            raise InvalidArgumentError("document_offsets and prefix_lengths cannot be combined")
-        if not isinstance(document_offsets, torch.Tensor) or document_offsets.dim() != 2 or document_offsets.shape[1] < 2:
-            raise InvalidArgumentError(f"document_offsets must have shape [{b}, documents + 1]")
-        _check_side("document_offsets", document_offsets, (b, document_offsets.shape[1]), torch.int32, query)
-        d.num_documents = document_offsets.shape[1] - 1
-        d.document_offsets = document_offsets.data_ptr() or None
-    if prefix_lengths is not None:
-        if not causal_mask:
-            raise InvalidArgumentError("prefix_lengths widens the causal mask: causal_mask must be set")
-        _check_side("prefix_lengths", prefix_lengths, (b,), torch.int32, query)
-        d.prefix_lengths = prefix_lengths.data_ptr() or None
-    _require_available()
-    if not query.is_cuda:
-        raise TypeError("query, key and value must be CUDA tensors")
-    query, key, value = _score_operand(query), _score_operand(key), _score_operand(value)
-    d.q, d.k, d.v = query.data_ptr(), key.data_ptr(), value.data_ptr()
-    _set_strides(d, "q_stride", query)
-    _set_strides(d, "k_stride", key)
-    _set_strides(d, "v_stride", value)
-    return d, query, key, value
-
-
-def _score_launch(entry: str, what: str, d, device: torch.device) -> None:
-    """Calls a descriptor-taking entry point on the current stream of `device`."""
-    d.stream = torch.cuda.current_stream(device).cuda_stream
-    fn = getattr(_b.load_library(), entry)
-    if device.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(d))
+def _score_launch(entry, what: str, d, index: int) -> None:
+    """Calls a descriptor-taking entry point with the device of the tensors current; its stream is already in the descriptor."""
+    if index == torch.cuda.current_device():
+        rc = entry(ctypes.byref(d))
     else:
-        with torch.cuda.device(device):
-            rc = fn(ctypes.byref(d))
+        with torch.cuda.device(index):
+            rc = entry(ctypes.byref(d))
     if rc == _b.CUDA_ERROR_INVALID_VALUE:
         raise InvalidArgumentError(f"{what} rejected its arguments (cudaErrorInvalidValue)")
     if rc != _b.CUDA_SUCCESS:
         raise InternalError(f"{what} failed: {_b.error_string(rc)}")
+
+
+def _score_workspace(entry, d, index: int) -> Optional[torch.Tensor]:
+    """Scratch from the caller's allocator for this call alone: two captured graphs, or two streams, never share it."""
+    if index == torch.cuda.current_device():
+        need = int(entry(ctypes.byref(d)))
+    else:
+        with torch.cuda.device(index):
+            need = int(entry(ctypes.byref(d)))
+    if not need:
+        return None
+    ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    return ws
 
 
 def _score_out(out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor:
@@ -933,6 +918,52 @@ def _score_out(out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor
     if out.shape != query.shape or (out.shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError(f"`out` must have shape {tuple(query.shape)} and a contiguous head dimension")
     return out
+
+
+def _score_sequence(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths, grad_out=None, out=None,
+                    lse=None):
+    """Checks the arguments of the sequence forms; returns the operands the kernels read and the descriptor's fields up to the
+    strides, but for out and lse."""
+    _check_query(query, 4, "query, key and value must be 4-dimensional [batch, heads, seq, head_dim]")
+    _check_same("key", key, query)
+    _check_same("value", value, query)
+    if key.dim() != 4 or value.dim() != 4:
+        raise ValueError("query, key and value must be 4-dimensional [batch, heads, seq, head_dim]")
+    b, h, sq, dim = query.shape
+    _, kv_heads, sk, _ = shape = key.shape
+    if shape != (b, kv_heads, sk, dim) or value.shape != shape:
+        raise InvalidArgumentError("query [B, H, Sq, D], key [B, Hk, Sk, D] and value [B, Hk, Sk, D] are required")
+    _check_heads(h, kv_heads, dim)
+    scale, softcap = _score_scalars(dim, scale, softcap)
+    if alibi_slopes is not None:
+        _check_side("alibi_slopes", alibi_slopes, (h,), torch.float32, query)
+    documents = 0
+    if document_offsets is not None:
+        if prefix_lengths is not None:
+            raise InvalidArgumentError("document_offsets and prefix_lengths cannot be combined")
+        if not isinstance(document_offsets, torch.Tensor) or document_offsets.dim() != 2 or document_offsets.shape[1] < 2:
+            raise InvalidArgumentError(f"document_offsets must have shape [{b}, documents + 1]")
+        documents = document_offsets.shape[1] - 1
+        _check_side("document_offsets", document_offsets, (b, documents + 1), torch.int32, query)
+    if prefix_lengths is not None:
+        if not causal_mask:
+            raise InvalidArgumentError("prefix_lengths widens the causal mask: causal_mask must be set")
+        _check_side("prefix_lengths", prefix_lengths, (b,), torch.int32, query)
+    if grad_out is not None:
+        for name, t in (("grad_out", grad_out), ("out", out)):
+            _check_same(name, t, query)
+            if t.shape != query.shape:
+                raise InvalidArgumentError(f"{name} must have the query's shape {tuple(query.shape)}, got {tuple(t.shape)}")
+        _check_side("lse", lse, (b, h, sq), torch.float32, query)
+    if not (_SM120_AVAILABLE and query.is_cuda):
+        _require_available()
+        raise TypeError("query, key and value must be CUDA tensors")
+    query, key, value = _score_operand(query), _score_operand(key), _score_operand(value)
+    head = (_TORCH_TO_SM120[query.dtype], 1 if causal_mask else 0, documents, b, h, kv_heads, sq, sk, dim, scale, softcap,
+            query.data_ptr(), key.data_ptr(), value.data_ptr())
+    side = (0 if alibi_slopes is None else alibi_slopes.data_ptr(), document_offsets.data_ptr() if documents else 0,
+            0 if prefix_lengths is None else prefix_lengths.data_ptr())
+    return query, key, value, head, side
 
 
 def score_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, scale: Optional[float] = None,
@@ -966,15 +997,13 @@ def score_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
     float16 / bfloat16 with D a multiple of 8 up to 128 run on the tensor cores; float32 and
     other D up to 256 on a plain kernel."""
-    d, query, key, value = _score_sequence_desc(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths)
+    query, key, value, head, side = _score_sequence(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths)
     out = _score_out(out, query)
-    d.out = out.data_ptr()
-    _set_strides(d, "out_stride", out)
-    lse = None
-    if return_lse:
-        lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device)
-        d.lse = lse.data_ptr() or None
-    _score_launch("sm120_launch_score_attention", "score_attention", d, query.device)
+    index = query.get_device()
+    lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device) if return_lse else None
+    d = _score_desc(*head, out.data_ptr(), lse.data_ptr() if return_lse else 0, *side, *query.stride()[:3], *key.stride()[:3], *value.stride()[:3],
+                    *out.stride()[:3], 0, 0, 0, 0, *_ZERO3, *_ZERO3, *_ZERO3, *_ZERO3, 0, 0, 0, 0, *_ZERO2, *_ZERO2, 0, 0, _raw_stream(index))
+    _score_launch(_b.load_library().sm120_launch_score_attention, "score_attention", d, index)
     return (out, lse) if return_lse else out
 
 
@@ -986,26 +1015,19 @@ def score_attention_grad(grad_out: torch.Tensor, query: torch.Tensor, key: torch
     options, from its result `out`, its `lse` and the result's gradient
     (``sm120_launch_score_attention_grad``).  Key and value gradients are summed over the query
     heads that share a key head, in a fixed order.  The slopes have no gradient."""
-    d, query, key, value = _score_sequence_desc(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths)
-    for name, t in (("grad_out", grad_out), ("out", out)):
-        _check_same(name, t, query)
-        if t.shape != query.shape:
-            raise InvalidArgumentError(f"{name} must have the query's shape {tuple(query.shape)}, got {tuple(t.shape)}")
-    _check_side("lse", lse, query.shape[:3], torch.float32, query)
+    if grad_out is None:
+        raise TypeError("grad_out must be a tensor")
+    query, key, value, head, side = _score_sequence(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths,
+                                                    grad_out, out, lse)
     out, grad_out = _score_operand(out), _score_operand(grad_out)
     dq, dk, dv = torch.empty_like(query), torch.empty_like(key), torch.empty_like(value)
-    d.out, d.lse, d.grad_out = out.data_ptr(), lse.data_ptr() or None, grad_out.data_ptr()
-    d.grad_q, d.grad_k, d.grad_v = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    _set_strides(d, "out_stride", out)
-    _set_strides(d, "grad_out_stride", grad_out)
-    _set_strides(d, "grad_q_stride", dq)
-    _set_strides(d, "grad_k_stride", dk)
-    _set_strides(d, "grad_v_stride", dv)
-    # scratch from the caller's allocator for this call alone: two captured graphs, or two streams, never share it
-    need = int(_b.load_library().sm120_score_attention_grad_workspace_bytes(ctypes.byref(d)))
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=query.device)
-    d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
-    _score_launch("sm120_launch_score_attention_grad", "score_attention_grad", d, query.device)
+    index, lib = query.get_device(), _b.load_library()
+    d = _score_desc(*head, out.data_ptr(), lse.data_ptr(), *side, *query.stride()[:3], *key.stride()[:3], *value.stride()[:3], *out.stride()[:3],
+                    grad_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *grad_out.stride()[:3], *dq.stride()[:3],
+                    *dk.stride()[:3], *dv.stride()[:3], 0, 0, 0, 0, *_ZERO2, *_ZERO2, 0, 0, _raw_stream(index))
+    ws = _score_workspace(lib.sm120_score_attention_grad_workspace_bytes, d, index)      # held until the launch is queued
+    _score_launch(lib.sm120_launch_score_attention_grad, "score_attention_grad", d, index)
+    del ws
     return dq, dk, dv
 
 
@@ -1039,55 +1061,47 @@ def score_attention_trainable(query: torch.Tensor, key: torch.Tensor, value: tor
 
 
 def _score_token(what: str, query, prefix_key, prefix_value, key_cache, value_cache, lengths, scale, softcap, alibi_slopes, return_lse, out):
-    if not isinstance(query, torch.Tensor):
-        raise TypeError("query must be a tensor")
-    if query.dtype not in _SCORE_DTYPES:
-        raise ValueError(f"dtype {query.dtype} is not supported (float32, float16, bfloat16)")
+    shapes = "query must be [batch, heads, head_dim], the caches [batch, key heads, seq, head_dim]"
+    _check_query(query, 3, shapes)
     _check_same("key_cache", key_cache, query)
     _check_same("value_cache", value_cache, query)
-    if query.dim() != 3 or key_cache.dim() != 4 or value_cache.dim() != 4:
-        raise ValueError("query must be [batch, heads, head_dim], the caches [batch, key heads, seq, head_dim]")
+    if key_cache.dim() != 4 or value_cache.dim() != 4:
+        raise ValueError(shapes)
     b, h, dim = query.shape
-    kv_heads, sk = key_cache.shape[1], key_cache.shape[2]
-    if tuple(key_cache.shape) != (b, kv_heads, sk, dim) or tuple(value_cache.shape) != (b, kv_heads, sk, dim):
+    _, kv_heads, sk, _ = shape = key_cache.shape
+    if shape != (b, kv_heads, sk, dim) or value_cache.shape != shape:
         raise InvalidArgumentError("query [B, H, D], key_cache [B, Hk, S, D] and value_cache [B, Hk, S, D] are required")
-    if h < 1 or kv_heads < 1 or h % kv_heads:
-        raise InvalidArgumentError(f"the number of query heads ({h}) must be a multiple of the number of key heads ({kv_heads})")
-    if not 1 <= dim <= 256:
-        raise InvalidArgumentError(f"head dimension {dim} is not supported (1 to 256)")
+    _check_heads(h, kv_heads, dim)
     _check_side("lengths", lengths, (b,), torch.int32, query)
-    d = _score_options(query, h, scale, softcap, alibi_slopes)
-    d.batch, d.heads, d.kv_heads, d.seq_q, d.seq_k = b, h, kv_heads, 1, sk
+    scale, softcap = _score_scalars(dim, scale, softcap)
+    if alibi_slopes is not None:
+        _check_side("alibi_slopes", alibi_slopes, (h,), torch.float32, query)
+    prefix = 0
     if prefix_key is not None:
         _check_same("prefix_key", prefix_key, query)
         _check_same("prefix_value", prefix_value, query)
-        if prefix_key.dim() != 3 or tuple(prefix_key.shape) != (kv_heads, prefix_key.shape[1], dim) or prefix_value.shape != prefix_key.shape:
+        if prefix_key.dim() != 3 or prefix_key.shape != (kv_heads, prefix_key.shape[1], dim) or prefix_value.shape != prefix_key.shape:
             raise InvalidArgumentError(f"prefix_key and prefix_value must have shape [{kv_heads}, prefix, {dim}]")
-    _require_available()
-    if not query.is_cuda:
+        prefix = prefix_key.shape[1]
+    if not (_SM120_AVAILABLE and query.is_cuda):
+        _require_available()
         raise TypeError("query and the caches must be CUDA tensors")
     query, key_cache, value_cache = _score_operand(query), _score_operand(key_cache), _score_operand(value_cache)
-    if prefix_key is not None and prefix_key.shape[1] > 0:
+    tail = (0, 0, 0, *_ZERO2, *_ZERO2)
+    if prefix:
         prefix_key, prefix_value = _score_operand(prefix_key), _score_operand(prefix_value)
-        d.prefix_k, d.prefix_v, d.prefix_len = prefix_key.data_ptr(), prefix_value.data_ptr(), prefix_key.shape[1]
-        _set_strides(d, "prefix_k_stride", prefix_key, 2)
-        _set_strides(d, "prefix_v_stride", prefix_value, 2)
+        tail = (prefix_key.data_ptr(), prefix_value.data_ptr(), prefix, *prefix_key.stride()[:2], *prefix_value.stride()[:2])
     out = _score_out(out, query)
-    d.q, d.k, d.v, d.out = query.data_ptr(), key_cache.data_ptr() or None, value_cache.data_ptr() or None, out.data_ptr()
-    d.q_stride[:2], d.out_stride[:2] = query.stride()[:2], out.stride()[:2]
-    _set_strides(d, "k_stride", key_cache)
-    _set_strides(d, "v_stride", value_cache)
-    d.key_lengths = lengths.data_ptr() or None
-    lse = None
-    if return_lse:
-        lse = torch.empty((b, h), dtype=torch.float32, device=query.device)
-        d.lse = lse.data_ptr() or None
-    need = int(_b.load_library().sm120_score_attention_decode_workspace_bytes(ctypes.byref(d)))
-    ws = None
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=query.device)      # for this call alone, as in score_attention_grad
-        d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    _score_launch("sm120_launch_score_attention_decode", what, d, query.device)
+    index, lib = query.get_device(), _b.load_library()
+    lse = torch.empty((b, h), dtype=torch.float32, device=query.device) if return_lse else None
+    d = _score_desc(_TORCH_TO_SM120[query.dtype], 0, 0, b, h, kv_heads, 1, sk, dim, scale, softcap, query.data_ptr(), key_cache.data_ptr(),
+                    value_cache.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                    0 if alibi_slopes is None else alibi_slopes.data_ptr(), 0, 0, *query.stride()[:2], 0, *key_cache.stride()[:3],
+                    *value_cache.stride()[:3], *out.stride()[:2], 0, 0, 0, 0, 0, *_ZERO3, *_ZERO3, *_ZERO3, *_ZERO3, lengths.data_ptr(), *tail,
+                    0, 0, _raw_stream(index))
+    ws = _score_workspace(lib.sm120_score_attention_decode_workspace_bytes, d, index)    # held until the launch is queued
+    _score_launch(lib.sm120_launch_score_attention_decode, what, d, index)
+    del ws
     return (out, lse) if return_lse else out
 
 

@@ -127,6 +127,22 @@ def test_token_forms_refuse(ops):
         ops.score_attention_decode(q, k, v, [1, 2])
 
 
+def test_packed_descriptor_has_the_structs_layout(binding):
+    """The one-call packing writes every field where the struct has it."""
+    pack, fields = binding.SCORE_ATTENTION_PACK, binding.SM120ScoreAttentionDesc._fields_
+    assert pack.size == ctypes.sizeof(binding.SM120ScoreAttentionDesc)
+    values, expect = [], []
+    for name, kind in fields:
+        count = getattr(kind, "_length_", 1)
+        own = [float(len(values) + i) if kind is ctypes.c_float else len(values) + i + 1 for i in range(count)]
+        values += own
+        expect.append((name, own if count > 1 else own[0]))
+    d = binding.SM120ScoreAttentionDesc.from_buffer(bytearray(pack.pack(*values)))
+    for name, want in expect:
+        got = getattr(d, name)
+        assert (list(got) if isinstance(want, list) else got) == want, name
+
+
 def test_needs_a_gpu(ops):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
