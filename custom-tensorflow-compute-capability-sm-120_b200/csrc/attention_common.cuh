@@ -188,6 +188,18 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return d;
 }
 
+// tanh(u) / u for |u| <= SA_TANH_RANGE as a polynomial in v = u^2 on the FMA pipe: the interpolant of degree 5 at the Chebyshev nodes of
+// [0, 0.64], off by at most 4e-8; with the roundings of an fp32 evaluation tanh is off by 1.1e-7, what 1 - 2 / (1 + e^2u) from the
+// MUFU unit gives as well.  Capped scores are rarely beyond: 0.8 is a score of 0.8 caps.
+constexpr float SA_TANH_RANGE = 0.8f;
+__device__ __forceinline__ uint64_t sa_tanh_ratio2(uint64_t v2) {
+    uint64_t r = fma2(v2, f32x2(-4.34973891e-3f, -4.34973891e-3f), f32x2(1.90843537e-2f, 1.90843537e-2f));
+    r = fma2(r, v2, f32x2(-5.3109269e-2f, -5.3109269e-2f));
+    r = fma2(r, v2, f32x2(0.133209318f, 0.133209318f));
+    r = fma2(r, v2, f32x2(-0.333326655f, -0.333326655f));
+    return fma2(r, v2, f32x2(0.999999941f, 0.999999941f));
+}
+
 // the three-input maximum / minimum of sm_100: half the instructions and half the chain length of a row's search
 __device__ __forceinline__ float att_max3(float a, float b, float c) {
     float d;

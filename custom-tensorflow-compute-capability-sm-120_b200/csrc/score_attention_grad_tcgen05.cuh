@@ -10,17 +10,24 @@
 // The two are one kernel, because they are the same with the roles of queries and keys exchanged:
 //                 rows (fixed, 128)      streamed (tiles of 64)     S = X U^T     dP = Y W^T     sums in TMEM
 //     KEYS        X = K,  Y = V          U = Q, W = grad_O          S^T           dP^T           A1 += dx^T U,  A2 += P^T W
-//     QUERIES     X = Q,  Y = grad_O     U = K, W = V               S             dP             A1 += dx U
+//     QUERIES     X = Q,  Y = grad_O     U = K, W = V               S             dP             A1 += dx U,  A2 += P (1 - tanh^2) U
+// QUERIES runs first and makes D exact.  D = <grad_O, O> of the prepare pass carries the rounding of O to 16 bits, which where few keys
+// dominate a row is as large as the rest of the error together.  The row's sum of P (dP - D) is what D lacks; it corrects grad_Q through A2
+// (grad_Q = scale (A1 - lack A2), one product more) and goes into neg_delta for the KEYS kernel.  Measured on peaked capped
+// scores (relative error of grad_Q, bf16, against 64 bits, 2 x 16 heads x 2048 causal, cap 30): 2.9e-3 before, 2.4e-3 with it, for 4 % of a training step's time.
 // Warp 0 feeds shared memory by TMA (X and Y once, U and W through a four-stage ring), warp 1 issues tcgen05.mma,
-// and two groups of four warps take alternate tiles: thread r of a group owns row r (TMEM lane r), reads its 64 scores and 64 dP,
-// and writes P and dx as packed 16-bit pairs over the first 32 cells of the two buffers it has just read, where they
-// are the A operands of the sums.  U and W serve both products of their kernel from one copy: rows of 128 swizzled bytes are K-major
+// and two groups of eight warps take alternate tiles: a thread owns half a row (TMEM lane, 32 of the 64 columns), reads its scores and dP,
+// and writes P and dx as packed 16-bit pairs over the first half of the columns it has just read, where they
+// are the A operands of the sums.  (Four warps per group, a whole row per thread: @@FOURWARPS@@ at 16 heads x 8192 x 128. What a group does between
+// two products is latency, not throughput: a quarter of the issue slots were used.)  U and W serve both products of their kernel from one copy: rows of 128 swizzled bytes are K-major
 // for S and dP and N-major for the sums.  Issue order ... A_j, S_{j+2}, dP_{j+2}, A_{j+1} ...: one thread's MMAs run in order, so the
 // buffers are free when the next scores overwrite them.  P and dx arrive in two halves of 32 streamed rows, so the first half's sums
 // start while the second is computed.
 // TMEM at D = 128: 2 x (64 + 64) scores and dP, 128 + 128 sums = 512 columns: no room for 128-row stream tiles.
 // What a row of the stream needs (neg_lse, neg_delta, its key range) comes with the tile in the KEYS kernel and sits in
 // registers in the other.
+
+#include <type_traits>
 
 #include "attention_common.cuh"
 #include "score_attention.h"
@@ -29,10 +36,15 @@ namespace sm120 {
 
 constexpr int SG_T = SA_GRAD_TILE;       // streamed rows per tile
 constexpr int SG_STAGES = 4;
+constexpr int SG_THREADS = 640;          // warp group 0: TMA, MMA and two idle warps; sixteen warps form P and dx
+constexpr int SG_REGS_LOW = 40, SG_REGS_HIGH = 104, SG_REGS_LAUNCH = 96;
+// as in attention_common.cuh: the sixteen warps may only ask for what warp group 0 gives back
+static_assert(16 * (SG_REGS_HIGH - SG_REGS_LAUNCH) <= 4 * (SG_REGS_LAUNCH - SG_REGS_LOW), "register hand-over does not balance");
+static_assert(SG_REGS_LAUNCH * SG_THREADS <= 65536, "register file");
 
 struct SaGradParams {
     ScoreParams s;
-    float scale_log2, cap_in, cap_log2;  // as in SaFwdParams
+    float scale_log2, cap_in, cap_log2, cap_u;           // as in SaFwdParams
     int bf16;
     unsigned long long wait_limit_ns;
     unsigned int* status;
@@ -47,7 +59,8 @@ struct SgCfg {
     static constexpr uint32_t STAGE_BYTES = 2 * U_BYTES;
     static constexpr uint32_t STAT_OFF = 2 * X_BYTES + SG_STAGES * STAGE_BYTES;
     static constexpr uint32_t BAR_OFF = STAT_OFF + SG_STAGES * STAT_BYTES;
-    static constexpr size_t SMEM_USED = BAR_OFF + 256 + 1024;
+    // barriers, what the four threads of a row tell each other (QUERIES)
+    static constexpr size_t SMEM_USED = BAR_OFF + 256 + 4 * ATT_BM * 4 + 1024;
     // every CTA allocates all 512 TMEM columns, so two CTAs must never share an SM: request more than half of its shared memory
     static constexpr size_t SMEM = SMEM_USED > 118784 ? SMEM_USED : 118784;
     static constexpr uint32_t TMEM_COLS = 512;
@@ -65,31 +78,41 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 // P and dx of 32 of a row's columns, packed.  Column c of the tile stands at distance rel + DIR * c (key position minus query
 // position; DIR = -1 where the columns are queries).  EDGE: columns outside the range count as 0 whatever they hold.
-// KEYS reads neg_lse, neg_delta and the ranges of the columns from shared memory; otherwise they belong to the row.
-template <bool KEYS, bool CAP, bool BIAS, bool EDGE>
+// KEYS reads neg_lse, neg_delta and the ranges of the columns from shared memory; otherwise they belong to the row, P comes out times
+// (1 - tanh^2), and the row's P (dP + neg_delta) is added to `lack`.
+// SMALL: every |score| is inside the range of the tanh polynomial.
+template <bool KEYS, bool CAP, bool BIAS, bool EDGE, bool SMALL>
 __device__ __forceinline__ void sg_chunk(const uint32_t (&s)[32], const uint32_t (&dp)[32], uint32_t (&pp)[16], uint32_t (&pd)[16], int c0,
                                          const SaGradParams& p, float slope_log2, float rel, int side, const float* col_lse, const float* col_delta,
-                                         const int2* col_range, float row_lse, float row_delta, uint32_t off0, uint32_t width) {
-    const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), in2 = f32x2(p.cap_in, p.cap_in), one2 = f32x2(1.0f, 1.0f),
+                                         const int2* col_range, float row_lse, float row_delta, uint32_t off0, uint32_t width, float& lack) {
+    const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), in2 = f32x2(p.cap_in, p.cap_in), small2 = f32x2(p.cap_u, p.cap_u), one2 = f32x2(1.0f, 1.0f),
                    cap2 = f32x2(p.cap_log2, p.cap_log2), minus2 = f32x2(-1.0f, -1.0f);
     const float dir = KEYS ? -1.0f : 1.0f;
     const float sl = side == SA_SIDE_BEFORE ? slope_log2 : -slope_log2;
-    const uint64_t sl2 = f32x2(sl, sl), step2 = f32x2(sl * dir, sl * dir), base2 = f32x2(sl * rel, sl * rel);
+    const float step = sl * dir, base = sl * rel;
+    uint64_t lack2 = f32x2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
         const int c = c0 + i;
         uint64_t add = KEYS ? *reinterpret_cast<const uint64_t*>(col_lse + c) : f32x2(row_lse, row_lse);
         if constexpr (BIAS) {
-            if (side != SA_SIDE_MIXED) add = add2(add, fma2(f32x2(static_cast<float>(c), static_cast<float>(c + 1)), step2, base2));
-            else add = fma2(f32x2(fabsf(rel + dir * static_cast<float>(c)), fabsf(rel + dir * static_cast<float>(c + 1))), sl2, add);
+            // scalar: the column is an immediate of the multiply-add
+            if (side != SA_SIDE_MIXED) add = add2(add, f32x2(fmaf(step, static_cast<float>(c), base), fmaf(step, static_cast<float>(c + 1), base)));
+            else add = add2(add, f32x2(sl * fabsf(rel + dir * static_cast<float>(c)), sl * fabsf(rel + dir * static_cast<float>(c + 1))));
         }
         const uint64_t x2 = f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         uint64_t z2, curve2 = 0;
         if constexpr (CAP) {
-            float a, b;
-            f32x2_split(mul2(x2, in2), a, b);
-            f32x2_split(add2(f32x2(att_exp2(a), att_exp2(b)), one2), a, b);
-            const uint64_t tanh2 = fma2(f32x2(att_rcp(a), att_rcp(b)), f32x2(-2.0f, -2.0f), one2);
+            uint64_t tanh2;
+            if constexpr (SMALL) {
+                const uint64_t u2 = mul2(x2, small2);
+                tanh2 = mul2(u2, sa_tanh_ratio2(mul2(u2, u2)));
+            } else {
+                float a, b;
+                f32x2_split(mul2(x2, in2), a, b);
+                f32x2_split(add2(f32x2(att_exp2(a), att_exp2(b)), one2), a, b);
+                tanh2 = fma2(f32x2(att_rcp(a), att_rcp(b)), f32x2(-2.0f, -2.0f), one2);
+            }
             z2 = fma2(tanh2, cap2, add);
             curve2 = fma2(mul2(tanh2, minus2), tanh2, one2);
         } else {
@@ -101,8 +124,10 @@ __device__ __forceinline__ void sg_chunk(const uint32_t (&s)[32], const uint32_t
         p1 = att_exp2(p1);
         uint64_t d2 = add2(f32x2(__uint_as_float(dp[i]), __uint_as_float(dp[i + 1])),
                            KEYS ? *reinterpret_cast<const uint64_t*>(col_delta + c) : f32x2(row_delta, row_delta));
-        if constexpr (CAP) d2 = mul2(d2, curve2);
-        f32x2_split(mul2(d2, f32x2(p0, p1)), d0, d1);
+        if constexpr (KEYS) {
+            if constexpr (CAP) d2 = mul2(d2, curve2);
+            f32x2_split(mul2(d2, f32x2(p0, p1)), d0, d1);
+        }
         if constexpr (EDGE) {
             bool in0, in1;
             if constexpr (KEYS) {
@@ -114,12 +139,37 @@ __device__ __forceinline__ void sg_chunk(const uint32_t (&s)[32], const uint32_t
                 in0 = off0 + c < width;
                 in1 = off0 + c + 1 < width;
             }
-            if (!in0) p0 = d0 = 0.0f;
-            if (!in1) p1 = d1 = 0.0f;
+            if constexpr (KEYS) {
+                if (!in0) p0 = d0 = 0.0f;
+                if (!in1) p1 = d1 = 0.0f;
+            } else {
+                // dP of a key outside the range may be anything as well
+                float e0, e1;
+                f32x2_split(d2, e0, e1);
+                if (!in0) p0 = e0 = 0.0f;
+                if (!in1) p1 = e1 = 0.0f;
+                d2 = f32x2(e0, e1);
+            }
         }
-        if constexpr (KEYS) pp[i >> 1] = pack16(p0, p1, p.bf16);
+        if constexpr (!KEYS) {
+            uint64_t p2 = f32x2(p0, p1);
+            if constexpr (CAP) {
+                lack2 = fma2(d2, p2, lack2);
+                p2 = mul2(p2, curve2);
+                d2 = mul2(d2, p2);
+                f32x2_split(p2, p0, p1);
+            } else {
+                d2 = mul2(d2, p2);
+                lack2 = add2(lack2, d2);
+            }
+            f32x2_split(d2, d0, d1);
+        }
+        pp[i >> 1] = pack16(p0, p1, p.bf16);
         pd[i >> 1] = pack16(d0, d1, p.bf16);
     }
+    float la, lb;
+    f32x2_split(lack2, la, lb);
+    lack += la + lb;
 }
 
 // Zeroes rows [r0, r1) of a stream tile's U and W and hands the writes to the async proxy.  One warp; it issues the products that read them.
@@ -135,7 +185,7 @@ __device__ __forceinline__ void sg_zero_rows(uint8_t* stage, int r0, int r1, int
 }
 
 template <int D, bool KEYS, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(ATT_THREADS, 1)
+__global__ void __launch_bounds__(SG_THREADS, 1)
 sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                   const __grid_constant__ CUtensorMap tmap_y,
                                   const __grid_constant__ CUtensorMap tmap_u,
@@ -159,6 +209,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
     volatile uint32_t* abort_flag = tmem_holder + 1;
     volatile int* stream_range = reinterpret_cast<volatile int*>(tmem_holder + 2);      // first streamed row, end
+    float* lacks = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);     // [group, half][ATT_BM]
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -243,7 +294,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     const int n_tiles = KEYS ? per_head * sp.group : per_head;
     const int head0 = KEYS ? rh * sp.group : kvh;                                        // head of the first streamed tile
 
-    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(ATT_REGS_LOW));
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SG_REGS_LOW));
 
     if (warp == 0) {
         // ------------------------------ TMA producer ------------------------------
@@ -311,11 +362,10 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                 if (t < t0 || t >= t1) continue;
                 const uint32_t acc = (t != 0 || j != 0) ? 1u : 0u;
                 const uint64_t u_desc = desc_hi | ((((u_smem + t * 2048) >> 4) & 0x3FFFu) | lbo_n);      // 16 rows of 128 bytes per K step
-                umma_ts_f16(a1, d_tmem + t * 8, u_desc, idesc_a, acc);
-                if (KEYS) {
-                    const uint64_t w_desc = desc_hi | ((((w_smem + t * 2048) >> 4) & 0x3FFFu) | lbo_n);
-                    umma_ts_f16(a2, p_tmem + t * 8, w_desc, idesc_a, acc);
-                }
+                const uint32_t cell = (t >> 1) * 32 + (t & 1) * 8;                                        // 16 rows = 8 cells of a half's 16
+                umma_ts_f16(a1, d_tmem + cell, u_desc, idesc_a, acc);
+                const uint64_t w_desc = desc_hi | ((((w_smem + t * 2048) >> 4) & 0x3FFFu) | lbo_n);
+                umma_ts_f16(a2, p_tmem + cell, KEYS ? w_desc : u_desc, idesc_a, acc);
             }
             if (t1 == SG_T / 16) {
                 umma_commit<1>(empty + 8 * st);
@@ -369,17 +419,17 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         }
     } else if (warp >= 4) {
         // ------------------------------ P, dx and output ------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(ATT_REGS_HIGH));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SG_REGS_HIGH));
         const int lane_group = warp & 3;
-        const int g = (warp - 4) >> 2;
+        const int g = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;      // group (tiles j % 2 == g), columns [32 * half, +32)
         const int row = lane_group * 32 + lane;
         const int r = r0 + row;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16);
-        const uint32_t t_s = t_lane + g * (2 * SG_T), t_d = t_s + SG_T;
+        const uint32_t t_s = t_lane + g * (2 * SG_T) + half * 32, t_d = t_s + SG_T;
         const bool pure_causal = sp.causal && sp.prefix_lengths == nullptr;
         // QUERIES: what belongs to the row
         int lo = 0, hi = 0;
-        float row_lse = 0.0f, row_delta = 0.0f, slope_log2 = 0.0f;
+        float row_lse = 0.0f, row_delta = 0.0f, slope_log2 = 0.0f, lack = 0.0f;
         if (!KEYS) {
             const int64_t at = (static_cast<int64_t>(b) * sp.heads + rh) * sp.seq_q_pad + min(r, sp.seq_q);      // row seq_q is padding: P = 0
             row_lse = sp.neg_lse[at];
@@ -412,17 +462,21 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             tcgen05_fence_after();
-            uint32_t s[SG_T], dp[SG_T];
+            uint32_t s[32], dp[32];
             __syncwarp();
+            tmem_ld_32x32(t_s, s);
+            tmem_ld_32x32(t_d, dp);
+            tmem_ld_wait_regs(s);
+            tmem_ld_wait_regs(dp);
+            bool small = false;
+            if constexpr (CAP) {
+                float top = __uint_as_float(s[0]), low = top;
 #pragma unroll
-            for (int c = 0; c < SG_T / 32; ++c) {
-                tmem_ld_32x32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-                tmem_ld_32x32(t_d + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&dp[c * 32]));
-            }
-#pragma unroll
-            for (int c = 0; c < SG_T / 32; ++c) {
-                tmem_ld_wait_regs(*reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-                tmem_ld_wait_regs(*reinterpret_cast<uint32_t(*)[32]>(&dp[c * 32]));
+                for (int i = 0; i < 32; i += 2) {
+                    top = att_max3(top, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    low = att_min3(low, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                }
+                small = __all_sync(0xFFFFFFFFu, fmaxf(top, -low) * fabsf(p.cap_u) <= SA_TANH_RANGE);
             }
             bool edge;
             uint32_t off0, width = 0;
@@ -443,22 +497,24 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                 rel = static_cast<float>(u0 - (r + first_pos));
                 side = pure_causal || u0 + SG_T - 1 <= r0 + first_pos ? SA_SIDE_BEFORE : u0 >= r0 + first_pos + ATT_BM - 1 ? SA_SIDE_BEHIND : SA_SIDE_MIXED;
             }
-#pragma unroll
-            for (int c = 0; c < SG_T / 32; ++c) {
-                uint32_t pp[16], pd[16];
-                const uint32_t(&sc)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&s[c * 32]);
-                const uint32_t(&dc)[32] = *reinterpret_cast<const uint32_t(*)[32]>(&dp[c * 32]);
-                if (edge)
-                    sg_chunk<KEYS, CAP, BIAS, true>(sc, dc, pp, pd, c * 32, p, slope_log2, rel, side, col_lse, col_delta, col_range, row_lse, row_delta, off0, width);
-                else
-                    sg_chunk<KEYS, CAP, BIAS, false>(sc, dc, pp, pd, c * 32, p, slope_log2, rel, side, col_lse, col_delta, col_range, row_lse, row_delta, off0, width);
-                if (KEYS) tmem_st_32x32(t_s + c * 16, pp);
-                tmem_st_32x32(t_d + c * 16, pd);
-                tmem_st_wait();
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive((c == 0 ? a_lo : a_hi) + 8 * g);
+            uint32_t pp[16], pd[16];
+            auto chunk = [&](auto on_edge, auto in_range) {
+                sg_chunk<KEYS, CAP, BIAS, decltype(on_edge)::value, decltype(in_range)::value>(s, dp, pp, pd, half * 32, p, slope_log2, rel, side, col_lse,
+                                                                                              col_delta, col_range, row_lse, row_delta, off0, width, lack);
+            };
+            if (CAP && small) {
+                if (edge) chunk(std::true_type{}, std::true_type{});
+                else chunk(std::false_type{}, std::true_type{});
+            } else {
+                if (edge) chunk(std::true_type{}, std::false_type{});
+                else chunk(std::false_type{}, std::false_type{});
             }
+            tmem_st_32x32(t_s, pp);
+            tmem_st_32x32(t_d, pd);
+            tmem_st_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive((half == 0 ? a_lo : a_hi) + 8 * g);
             next_tile();
             if (j + 2 < n_tiles) next_tile();
         }
@@ -466,37 +522,51 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             ok = att_wait(sums_done, 0u, wctx, 0x64000000u);
             ok = __all_sync(0xFFFFFFFFu, ok);
         }
+        if (!KEYS) {
+            // what D lacks, from the row's four threads in one order.  Every one of the sixteen warps comes here, aborted or not.
+            lacks[(g * 2 + half) * ATT_BM + row] = lack;
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            lack = (lacks[row] + lacks[ATT_BM + row]) + (lacks[2 * ATT_BM + row] + lacks[3 * ATT_BM + row]);
+            if (ok && g == 0 && half == 0 && r < rows && row_lse != -CUDART_INF_F)
+                sp.neg_delta[(static_cast<int64_t>(b) * sp.heads + rh) * sp.seq_q_pad + r] = row_delta - lack;
+        }
         if (ok) {
-            constexpr int HD = D / 2;                           // this thread writes columns [g * HD, +HD) of its row
-            const int head_out = rh;
+            constexpr int CW = D / 4;                           // this thread writes columns [col, +CW) of its row
+            const int col = (g * 2 + half) * CW;
             tcgen05_fence_after();
 #pragma unroll
             for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
                 void* base = KEYS ? (which == 0 ? sp.grad_k : sp.grad_v) : sp.grad_q;
                 const int64_t* st = KEYS ? (which == 0 ? sp.gk_st : sp.gv_st) : sp.gq_st;
                 const float factor = which == 0 ? sp.scale : 1.0f;
-                uint16_t* dst = static_cast<uint16_t*>(base) + b * st[0] + head_out * st[1] + r * st[2];
+                uint16_t* dst = static_cast<uint16_t*>(base) + b * st[0] + rh * st[1] + r * st[2];
+                uint32_t o[CW];
+                auto load_sums = [&](uint32_t taddr, uint32_t (&v)[CW]) {
+                    if constexpr (CW == 32) tmem_ld_32x32_sync(taddr, v);
+                    else tmem_ld_32x16_sync(taddr, v);
+                };
+                if (n_tiles > 0) {
+                    __syncwarp();
+                    load_sums(t_lane + Cfg::TMEM_A + which * D + col, o);
+                    if (!KEYS) {
+                        uint32_t o2[CW];
+                        load_sums(t_lane + Cfg::TMEM_A + D + col, o2);
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t o[32];
-                    const int col = g * HD + c * 32;
-                    if (n_tiles > 0) {
-                        __syncwarp();
-                        tmem_ld_32x32_sync(t_lane + Cfg::TMEM_A + which * D + col, o);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = 0u;
+                        for (int i = 0; i < CW; ++i) o[i] = __float_as_uint(fmaf(-lack, __uint_as_float(o2[i]), __uint_as_float(o[i])));
                     }
-                    if (r < rows) {
+                } else {
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            if (col + v * 8 >= sp.head_dim) continue;     // head_dim is a multiple of 8
-                            uint32_t w[4];
+                    for (int i = 0; i < CW; ++i) o[i] = 0u;
+                }
+                if (r < rows) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = pack16(__uint_as_float(o[v * 8 + 2 * k]) * factor, __uint_as_float(o[v * 8 + 2 * k + 1]) * factor, p.bf16);
-                            *reinterpret_cast<uint4*>(dst + col + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                    for (int v = 0; v < CW / 8; ++v) {
+                        if (col + v * 8 >= sp.head_dim) continue;     // head_dim is a multiple of 8
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            w[k] = pack16(__uint_as_float(o[v * 8 + 2 * k]) * factor, __uint_as_float(o[v * 8 + 2 * k + 1]) * factor, p.bf16);
+                        *reinterpret_cast<uint4*>(dst + col + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
@@ -521,16 +591,16 @@ cudaError_t sa_grad_variant(const CUtensorMap& tx, const CUtensorMap& ty, const 
     auto kern = sm120_score_attention_grad_kernel<D, KEYS, CAP, BIAS>;
     const uint64_t bit = 1ull << (device & 63);
     if ((attr_done.load(std::memory_order_acquire) & bit) == 0) {
-        // the register hand-over inside the kernel balances only if the kernel starts with ATT_REGS_LAUNCH registers
+        // the register hand-over inside the kernel balances only if the kernel starts with SG_REGS_LAUNCH registers
         cudaFuncAttributes fa{};
         cudaError_t e = cudaFuncGetAttributes(&fa, kern);
         if (e != cudaSuccess) return e;
-        if (fa.numRegs != ATT_REGS_LAUNCH) return cudaErrorLaunchOutOfResources;
+        if (fa.numRegs != SG_REGS_LAUNCH) return cudaErrorLaunchOutOfResources;
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SgCfg<D>::SMEM));
         if (e != cudaSuccess) return e;
         attr_done.fetch_or(bit, std::memory_order_release);
     }
-    kern<<<grid, ATT_THREADS, SgCfg<D>::SMEM, stream>>>(tx, ty, tu, tw, p);
+    kern<<<grid, SG_THREADS, SgCfg<D>::SMEM, stream>>>(tx, ty, tu, tw, p);
     return cudaGetLastError();
 }
 

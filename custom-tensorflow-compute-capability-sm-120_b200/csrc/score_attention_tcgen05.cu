@@ -26,6 +26,7 @@ static void sa_fwd_constants(SaFwdParams& fp, const ScoreParams& p, int device) 
     fp.scale_log2 = p.scale * SA_LOG2E;
     fp.cap_in = p.softcap > 0.0f ? 2.0f * SA_LOG2E * p.scale / p.softcap : 0.0f;
     fp.cap_log2 = p.softcap * SA_LOG2E;
+    fp.cap_u = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
     fp.out_bf16 = p.dtype == SM120_DTYPE_BFLOAT16 ? 1 : 0;
     fp.wait_limit_ns = launch_wait_limit_ns();
     fp.status = tc_status_address(device);
@@ -89,6 +90,7 @@ cudaError_t sa_tc_grad(const ScoreParams& p, int device, cudaStream_t stream) {
     gp.scale_log2 = p.scale * SA_LOG2E;
     gp.cap_in = p.softcap > 0.0f ? 2.0f * SA_LOG2E * p.scale / p.softcap : 0.0f;
     gp.cap_log2 = p.softcap * SA_LOG2E;
+    gp.cap_u = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
     gp.bf16 = p.dtype == SM120_DTYPE_BFLOAT16 ? 1 : 0;
     gp.wait_limit_ns = launch_wait_limit_ns();
     gp.status = tc_status_address(device);

@@ -10,7 +10,8 @@
 //     per-row ranges whose ends never decrease), so its tiles start exactly at kv_lo and no tile outside is touched;
 //     a tile tests single keys only when some row's range ends inside it (one vote per warp).
 //   * Scores.  The cap and the distance bias are applied to the 128 scores in registers before the maximum:
-//     tanh(u) = 1 - 2 / (1 + e^2u), two more MUFU operations a score (ex2, rcp) next to the softmax's one; the bias
+//     tanh(u) as a polynomial on packed FMAs while a row's scores of the tile are within 0.8 caps, else 1 - 2 / (1 + e^2u), two more
+//     MUFU operations a score (ex2, rcp) next to the softmax's one, which then bound the tile (@@CAPTIMES@@); the bias
 //     is one packed multiply-add, because on one side of the query it is linear in the key index (the tile across
 //     the diagonal of a bidirectional mask takes the absolute value key by key).  Everything is in log2 units.
 //   * Tensors.  4-D tensor maps take any strides; query head h reads key head h / group.  Columns behind head_dim
@@ -31,6 +32,7 @@ struct SaFwdParams {
     float scale_log2;                // scale * log2(e)
     float cap_in;                    // 2 * log2(e) * scale / softcap: e^2u = 2^(dot * cap_in)
     float cap_log2;                  // softcap * log2(e)
+    float cap_u;                     // scale / softcap: u = dot * cap_u
     int out_bf16;
     // TOKEN
     int batch_per_tile;              // entries per 128-row tile: 128 / group
@@ -59,22 +61,26 @@ struct SaCfg {
 };
 
 // The scores of one row against ATT_BN keys: raw products in, log2-unit modified scores out.  `rel` is the first key's
-// position minus the query's.
-template <bool CAP, bool BIAS>
-__device__ __forceinline__ void sa_modify(uint32_t (&s)[ATT_BN], float scale_log2, float cap_in, float cap_log2, float slope_log2, float rel, int side) {
+// position minus the query's.  With BIAS the tile's keys lie on one side of the query and `slope_log2` has that side's sign, or
+// (MIXED) it is negative and the distance is taken key by key.
+// The bias is scalar arithmetic: the key's index is then an immediate of the multiply-add, a packed one would first have to be moved to registers.
+template <bool BIAS, bool MIXED>
+__device__ __forceinline__ uint64_t sa_bias2(int i, float sl, float base, float rel) {
+    if constexpr (!BIAS) return 0;
+    else if constexpr (MIXED) return f32x2(sl * fabsf(rel + static_cast<float>(i)), sl * fabsf(rel + static_cast<float>(i + 1)));
+    else return f32x2(fmaf(sl, static_cast<float>(i), base), fmaf(sl, static_cast<float>(i + 1), base));
+}
+template <bool CAP, bool BIAS, bool MIXED>
+__device__ __forceinline__ void sa_modify(uint32_t (&s)[ATT_BN], float scale_log2, float cap_in, float cap_log2, float sl, float rel) {
     const uint64_t one2 = f32x2(1.0f, 1.0f), in2 = f32x2(cap_in, cap_in), cap2 = f32x2(cap_log2, cap_log2),
                    ncap2 = f32x2(-2.0f * cap_log2, -2.0f * cap_log2), scale2 = f32x2(scale_log2, scale_log2);
-    const float sl = side == SA_SIDE_BEFORE ? slope_log2 : -slope_log2;
-    const uint64_t sl2 = f32x2(sl, sl), base2 = f32x2(sl * rel, sl * rel);
+    const float base = sl * rel;
 #pragma unroll
     for (int i = 0; i < ATT_BN; i += 2) {
-        uint64_t x2 = f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), b2 = 0;
-        if constexpr (BIAS) {
-            if (side != SA_SIDE_MIXED) b2 = fma2(f32x2(static_cast<float>(i), static_cast<float>(i + 1)), sl2, base2);
-            else b2 = mul2(f32x2(fabsf(rel + static_cast<float>(i)), fabsf(rel + static_cast<float>(i + 1))), sl2);
-        }
+        uint64_t x2 = f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        const uint64_t b2 = sa_bias2<BIAS, MIXED>(i, sl, base, rel);
+        float a, b;
         if constexpr (CAP) {
-            float a, b;
             f32x2_split(mul2(x2, in2), a, b);
             f32x2_split(add2(f32x2(att_exp2(a), att_exp2(b)), one2), a, b);
             x2 = fma2(f32x2(att_rcp(a), att_rcp(b)), ncap2, cap2);
@@ -82,11 +88,29 @@ __device__ __forceinline__ void sa_modify(uint32_t (&s)[ATT_BN], float scale_log
         } else {
             x2 = fma2(x2, scale2, b2);
         }
-        float a, b;
         f32x2_split(x2, a, b);
         s[i] = __float_as_uint(a);
         s[i + 1] = __float_as_uint(b);
     }
+}
+
+// The capped form for scores within the range of the tanh polynomial.  Returns the largest u^2: above SA_TANH_RANGE^2 the result is not used.
+template <bool BIAS, bool MIXED>
+__device__ __forceinline__ float sa_modify_small(uint32_t (&s)[ATT_BN], float cap_u, float cap_log2, float sl, float rel) {
+    const uint64_t in2 = f32x2(cap_u, cap_u), cap2 = f32x2(cap_log2, cap_log2);
+    const float base = sl * rel;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ATT_BN; i += 2) {
+        const uint64_t u2 = mul2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), in2), v2 = mul2(u2, u2);
+        float a, b;
+        f32x2_split(v2, a, b);
+        top = att_max3(top, a, b);
+        f32x2_split(fma2(mul2(u2, cap2), sa_tanh_ratio2(v2), sa_bias2<BIAS, MIXED>(i, sl, base, rel)), a, b);
+        s[i] = __float_as_uint(a);
+        s[i + 1] = __float_as_uint(b);
+    }
+    return top;
 }
 
 // p = exp2(s * scale2 + neg_m2) (MODIFIED scores already carry the scale) for KEYS keys, packed as 16-bit pairs, added to the
@@ -456,12 +480,24 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
             const uint32_t off0 = static_cast<uint32_t>(key0 - lo);          // wraps for keys before the range: larger than any width
             if constexpr (MODIFIED) {
                 const float rel = static_cast<float>(key0 - pos);
-                if constexpr (BIAS) {
-                    if (key0 + ATT_BN - 1 <= side_first) sa_modify<CAP, true>(s, scale_log2, p.cap_in, p.cap_log2, slope_log2, rel, SA_SIDE_BEFORE);
-                    else if (key0 >= side_last) sa_modify<CAP, true>(s, scale_log2, p.cap_in, p.cap_log2, slope_log2, rel, SA_SIDE_BEHIND);
-                    else sa_modify<CAP, true>(s, scale_log2, p.cap_in, p.cap_log2, slope_log2, rel, SA_SIDE_MIXED);
+                const bool before = !BIAS || key0 + ATT_BN - 1 <= side_first, mixed = BIAS && !before && key0 < side_last;
+                const float sl = before ? slope_log2 : -slope_log2;
+                if constexpr (CAP) {
+                    float top;
+                    if (mixed) top = sa_modify_small<BIAS, true>(s, p.cap_u, p.cap_log2, sl, rel);
+                    else top = sa_modify_small<BIAS, false>(s, p.cap_u, p.cap_log2, sl, rel);
+                    if (!__all_sync(0xFFFFFFFFu, top <= SA_TANH_RANGE * SA_TANH_RANGE)) {
+                        // a score of this warp's rows is too large: once more from the products, which still lie in TMEM
+#pragma unroll
+                        for (int c = 0; c < ATT_BN / 32; ++c) tmem_ld_32x32(t_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+#pragma unroll
+                        for (int c = 0; c < ATT_BN / 32; ++c) tmem_ld_wait_regs(*reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+                        // key by key holds on every side
+                        sa_modify<true, BIAS, true>(s, scale_log2, p.cap_in, p.cap_log2, -slope_log2, rel);
+                    }
                 } else {
-                    sa_modify<CAP, false>(s, scale_log2, p.cap_in, p.cap_log2, 0.0f, 0.0f, SA_SIDE_BEFORE);
+                    if (mixed) sa_modify<false, BIAS, true>(s, scale_log2, p.cap_in, p.cap_log2, sl, rel);
+                    else sa_modify<false, BIAS, false>(s, scale_log2, p.cap_in, p.cap_log2, sl, rel);
                 }
             }
             float m_tile;
