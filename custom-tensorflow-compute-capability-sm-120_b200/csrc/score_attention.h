@@ -13,10 +13,6 @@ constexpr float SA_LN2 = 0.69314718055994531f;
 constexpr int SA_ROW_PAD = 128;      // per-row arrays in the workspace have rows behind the last: a copy of SA_GRAD_TILE rows from any row stays inside
 constexpr int SA_GRAD_TILE = 64;     // streamed rows per tile of the gradient kernels
 
-// Which formula the distance bias of a tile takes: every key at or before every query (or masked), every key at or
-// behind, or key by key
-enum : int { SA_SIDE_BEFORE = 0, SA_SIDE_BEHIND = 1, SA_SIDE_MIXED = 2 };
-
 struct ScoreParams {
     int batch, heads, kv_heads, group;         // group = heads / kv_heads
     int seq_q, seq_k, head_dim, dtype;

@@ -18,11 +18,13 @@
 // Warp 0 feeds shared memory by TMA (X and Y once, U and W through a four-stage ring), warp 1 issues tcgen05.mma,
 // and two groups of eight warps take alternate tiles: a thread owns half a row (TMEM lane, 32 of the 64 columns), reads its scores and dP,
 // and writes P and dx as packed 16-bit pairs over the first half of the columns it has just read, where they
-// are the A operands of the sums.  (Four warps per group, a whole row per thread: @@FOURWARPS@@ at 16 heads x 8192 x 128. What a group does between
-// two products is latency, not throughput: a quarter of the issue slots were used.)  U and W serve both products of their kernel from one copy: rows of 128 swizzled bytes are K-major
+// are the A operands of the sums.  (Four warps per group, a whole row per thread: 2136 instead of 2094 us at 16 heads x 8192 x 128.)  U and W serve both products of their kernel from one copy: rows of 128 swizzled bytes are K-major
 // for S and dP and N-major for the sums.  Issue order ... A_j, S_{j+2}, dP_{j+2}, A_{j+1} ...: one thread's MMAs run in order, so the
-// buffers are free when the next scores overwrite them.  P and dx arrive in two halves of 32 streamed rows, so the first half's sums
-// start while the second is computed.
+// buffers are free when the next scores overwrite them.  A tile's sums and the scores two tiles on are issued in one go: the
+// issuing warp's wait and election cost 150 to 230 cycles of each tile's ~1800, so there is one of them (P and dx handed over in two halves, the
+// first half's sums under the second's arithmetic: 1554 instead of 1402 us at 16 heads x 8192 x 64, the same at head size 128).
+// What bounds it at D = 128 (cycle stamps): the tensor pipe.  A tile's sums take 8 x 64 cycles, its scores 16 x 80: an MMA whose A operand comes
+// from shared memory pays 64 cycles for its 4 KB whatever N is, and TMEM has no room for X and Y beside double-buffered scores.
 // TMEM at D = 128: 2 x (64 + 64) scores and dP, 128 + 128 sums = 512 columns: no room for 128-row stream tiles.
 // What a row of the stream needs (neg_lse, neg_delta, its key range) comes with the tile in the KEYS kernel and sits in
 // registers in the other.
@@ -76,6 +78,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
+// The bias is linear in the column where all keys of a tile lie on one side of all its queries; tiles across the diagonal take the EDGE form,
+// which forms the distance column by column.
 // P and dx of 32 of a row's columns, packed.  Column c of the tile stands at distance rel + DIR * c (key position minus query
 // position; DIR = -1 where the columns are queries).  EDGE: columns outside the range count as 0 whatever they hold.
 // KEYS reads neg_lse, neg_delta and the ranges of the columns from shared memory; otherwise they belong to the row, P comes out times
@@ -83,12 +87,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // SMALL: every |score| is inside the range of the tanh polynomial.
 template <bool KEYS, bool CAP, bool BIAS, bool EDGE, bool SMALL>
 __device__ __forceinline__ void sg_chunk(const uint32_t (&s)[32], const uint32_t (&dp)[32], uint32_t (&pp)[16], uint32_t (&pd)[16], int c0,
-                                         const SaGradParams& p, float slope_log2, float rel, int side, const float* col_lse, const float* col_delta,
+                                         const SaGradParams& p, float slope_log2, float rel, bool before, const float* col_lse, const float* col_delta,
                                          const int2* col_range, float row_lse, float row_delta, uint32_t off0, uint32_t width, float& lack) {
     const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), in2 = f32x2(p.cap_in, p.cap_in), small2 = f32x2(p.cap_u, p.cap_u), one2 = f32x2(1.0f, 1.0f),
                    cap2 = f32x2(p.cap_log2, p.cap_log2), minus2 = f32x2(-1.0f, -1.0f);
     const float dir = KEYS ? -1.0f : 1.0f;
-    const float sl = side == SA_SIDE_BEFORE ? slope_log2 : -slope_log2;
+    const float sl = before ? slope_log2 : -slope_log2;
     const float step = sl * dir, base = sl * rel;
     uint64_t lack2 = f32x2(0.0f, 0.0f);
 #pragma unroll
@@ -97,8 +101,8 @@ __device__ __forceinline__ void sg_chunk(const uint32_t (&s)[32], const uint32_t
         uint64_t add = KEYS ? *reinterpret_cast<const uint64_t*>(col_lse + c) : f32x2(row_lse, row_lse);
         if constexpr (BIAS) {
             // scalar: the column is an immediate of the multiply-add
-            if (side != SA_SIDE_MIXED) add = add2(add, f32x2(fmaf(step, static_cast<float>(c), base), fmaf(step, static_cast<float>(c + 1), base)));
-            else add = add2(add, f32x2(sl * fabsf(rel + dir * static_cast<float>(c)), sl * fabsf(rel + dir * static_cast<float>(c + 1))));
+            if constexpr (EDGE) add = add2(add, f32x2(-slope_log2 * fabsf(rel + dir * static_cast<float>(c)), -slope_log2 * fabsf(rel + dir * static_cast<float>(c + 1))));
+            else add = add2(add, f32x2(fmaf(step, static_cast<float>(c), base), fmaf(step, static_cast<float>(c + 1), base)));
         }
         const uint64_t x2 = f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         uint64_t z2, curve2 = 0;
@@ -202,8 +206,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     const uint32_t full = smem_u32(bars + 1);        // [4]
     const uint32_t empty = smem_u32(bars + 5);       // [4]
     const uint32_t s_full = smem_u32(bars + 9);      // [2]  S_j and dP_j are complete in TMEM (and with them every product issued before)
-    const uint32_t a_lo = smem_u32(bars + 11);       // [2]  S_j and dP_j have been read, columns 0-31 of P_j and dx_j are in TMEM
-    const uint32_t a_hi = smem_u32(bars + 13);       // [2]  columns 32-63
+    const uint32_t a_ready = smem_u32(bars + 11);    // [2]  S_j and dP_j have been read, P_j and dx_j are in TMEM
     const uint32_t sums_done = smem_u32(bars + 15);
     const uint32_t drain_bar = smem_u32(bars + 16);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
@@ -251,8 +254,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(s_full + 8 * g, 1);
-            mbar_init(a_lo + 8 * g, 4);              // one arrival per warp of the group
-            mbar_init(a_hi + 8 * g, 4);
+            mbar_init(a_ready + 8 * g, 8);           // one arrival per warp of the group
         }
         mbar_init(sums_done, 1);
         mbar_init(drain_bar, 1);
@@ -351,15 +353,14 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             }
             umma_commit<1>(s_full + 8 * g);
         };
-        // streamed rows 16 t0 .. 16 t1 into the sums (one elected thread)
-        auto sum_mmas = [&](int j, int t0, int t1) {
+        // the tile's rows into the sums (one elected thread)
+        auto sum_mmas = [&](int j) {
             const uint32_t st = j % SG_STAGES, g = j & 1;
             const uint32_t u_smem = ring + st * Cfg::STAGE_BYTES, w_smem = u_smem + Cfg::U_BYTES;
             const uint32_t p_tmem = tmem_base + g * (2 * SG_T), d_tmem = p_tmem + SG_T;
             const uint32_t a1 = tmem_base + Cfg::TMEM_A, a2 = a1 + D;
 #pragma unroll
             for (int t = 0; t < SG_T / 16; ++t) {
-                if (t < t0 || t >= t1) continue;
                 const uint32_t acc = (t != 0 || j != 0) ? 1u : 0u;
                 const uint64_t u_desc = desc_hi | ((((u_smem + t * 2048) >> 4) & 0x3FFFu) | lbo_n);      // 16 rows of 128 bytes per K step
                 const uint32_t cell = (t >> 1) * 32 + (t & 1) * 8;                                        // 16 rows = 8 cells of a half's 16
@@ -367,10 +368,8 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                 const uint64_t w_desc = desc_hi | ((((w_smem + t * 2048) >> 4) & 0x3FFFu) | lbo_n);
                 umma_ts_f16(a2, p_tmem + cell, KEYS ? w_desc : u_desc, idesc_a, acc);
             }
-            if (t1 == SG_T / 16) {
-                umma_commit<1>(empty + 8 * st);
-                if (j == n_tiles - 1) umma_commit<1>(sums_done);
-            }
+            umma_commit<1>(empty + 8 * st);
+            if (j == n_tiles - 1) umma_commit<1>(sums_done);
         };
         // rows of tile j that lie inside the tensor but outside [u_lo, u_hi) become zeros (behind the tensor TMA has filled in zeros)
         int clean_t = 0;                                       // tile index inside its head
@@ -394,20 +393,15 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         for (int j = 0; ok && j < n_tiles; ++j) {
             const uint32_t g = j & 1, ph = (j >> 1) & 1;
             const bool more = j + 2 < n_tiles;
-            bool w = att_wait(a_lo + 8 * g, ph, wctx, 0x54000000u);
-            ok = __all_sync(0xFFFFFFFFu, w);
-            if (!ok) break;
-            tcgen05_fence_after();
-            if (elect_one_sync()) sum_mmas(j, 0, SG_T / 32);
-            __syncwarp();
-            if (more) w = att_wait2(a_hi + 8 * g, ph, full + 8 * ((j + 2) % SG_STAGES), ((j + 2) / SG_STAGES) & 1, wctx, 0x55000000u, 0x52000000u);
-            else w = att_wait(a_hi + 8 * g, ph, wctx, 0x55000000u);
+            bool w;
+            if (more) w = att_wait2(a_ready + 8 * g, ph, full + 8 * ((j + 2) % SG_STAGES), ((j + 2) / SG_STAGES) & 1, wctx, 0x54000000u, 0x52000000u);
+            else w = att_wait(a_ready + 8 * g, ph, wctx, 0x54000000u);
             ok = __all_sync(0xFFFFFFFFu, w);
             if (!ok) break;
             if (more) clean(j + 2);
             tcgen05_fence_after();
             if (elect_one_sync()) {
-                sum_mmas(j, SG_T / 32, SG_T / 16);
+                sum_mmas(j);
                 if (more) score_mmas(j + 2);
             }
             __syncwarp();
@@ -426,7 +420,6 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         const int r = r0 + row;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16);
         const uint32_t t_s = t_lane + g * (2 * SG_T) + half * 32, t_d = t_s + SG_T;
-        const bool pure_causal = sp.causal && sp.prefix_lengths == nullptr;
         // QUERIES: what belongs to the row
         int lo = 0, hi = 0;
         float row_lse = 0.0f, row_delta = 0.0f, slope_log2 = 0.0f, lack = 0.0f;
@@ -481,7 +474,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             bool edge;
             uint32_t off0, width = 0;
             float rel;
-            int side;
+            bool before = true;
             if (KEYS) {
                 // the tile's first and last row bound every row's range
                 const int2 first = col_range[0], last = col_range[min(SG_T, sp.seq_q - u0) - 1];
@@ -489,17 +482,23 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                 edge = last.x > w0 || first.y < w0 + 32;
                 off0 = static_cast<uint32_t>(r);
                 rel = static_cast<float>(r - (u0 + first_pos));
-                side = pure_causal || r0 + ATT_BM - 1 <= u0 + first_pos ? SA_SIDE_BEFORE : r0 >= u0 + first_pos + SG_T - 1 ? SA_SIDE_BEHIND : SA_SIDE_MIXED;
+                if (BIAS) {
+                    before = r0 + ATT_BM - 1 <= u0 + first_pos;
+                    edge = edge || (!before && r0 < u0 + first_pos + SG_T - 1);
+                }
             } else {
                 edge = __any_sync(0xFFFFFFFFu, u0 < lo || u0 + SG_T > hi);
                 off0 = static_cast<uint32_t>(u0 - lo);
                 width = static_cast<uint32_t>(hi - lo);
                 rel = static_cast<float>(u0 - (r + first_pos));
-                side = pure_causal || u0 + SG_T - 1 <= r0 + first_pos ? SA_SIDE_BEFORE : u0 >= r0 + first_pos + ATT_BM - 1 ? SA_SIDE_BEHIND : SA_SIDE_MIXED;
+                if (BIAS) {
+                    before = u0 + SG_T - 1 <= r0 + first_pos;
+                    edge = edge || (!before && u0 < r0 + first_pos + ATT_BM - 1);
+                }
             }
             uint32_t pp[16], pd[16];
             auto chunk = [&](auto on_edge, auto in_range) {
-                sg_chunk<KEYS, CAP, BIAS, decltype(on_edge)::value, decltype(in_range)::value>(s, dp, pp, pd, half * 32, p, slope_log2, rel, side, col_lse,
+                sg_chunk<KEYS, CAP, BIAS, decltype(on_edge)::value, decltype(in_range)::value>(s, dp, pp, pd, half * 32, p, slope_log2, rel, before, col_lse,
                                                                                               col_delta, col_range, row_lse, row_delta, off0, width, lack);
             };
             if (CAP && small) {
@@ -514,7 +513,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             tmem_st_wait();
             tcgen05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive((half == 0 ? a_lo : a_hi) + 8 * g);
+            if (lane == 0) mbar_arrive(a_ready + 8 * g);
             next_tile();
             if (j + 2 < n_tiles) next_tile();
         }
