@@ -70,7 +70,8 @@ cudaError_t resolve(const SM120ScoreAttentionDesc* d, Form form, ScoreParams* p,
 // the three arrays of the gradient workspace; seq_q_pad keeps each a multiple of 16 bytes
 size_t stats_bytes(const ScoreParams& p) { return static_cast<size_t>(p.batch) * p.heads * p.seq_q_pad * sizeof(float); }
 size_t ranges_bytes(const ScoreParams& p) { return static_cast<size_t>(p.batch) * p.seq_q_pad * sizeof(int2); }
-size_t grad_workspace(const ScoreParams& p) { return 2 * stats_bytes(p) + ranges_bytes(p); }
+size_t row_bytes(const ScoreParams& p) { return 2 * stats_bytes(p) + ranges_bytes(p); }
+size_t grad_workspace(const ScoreParams& p, int sms) { return row_bytes(p) + (sa_tc_grad_supported(p) ? sa_tc_grad_workspace(p, sms) : 0); }
 
 bool workspace_ok(const SM120ScoreAttentionDesc* d, size_t need) {
     return need == 0 || (d->workspace != nullptr && (reinterpret_cast<uintptr_t>(d->workspace) & 15u) == 0 && d->workspace_bytes >= need);
@@ -108,8 +109,9 @@ cudaError_t sm120_launch_score_attention(const SM120ScoreAttentionDesc* desc) {
 size_t sm120_score_attention_grad_workspace_bytes(const SM120ScoreAttentionDesc* desc) {
     ScoreParams p{};
     bool empty = false;
-    if (resolve(desc, Form::GRADIENT, &p, &empty) != cudaSuccess || empty) return 0;
-    return grad_workspace(p);
+    int device = 0, sms = 0;
+    if (resolve(desc, Form::GRADIENT, &p, &empty) != cudaSuccess || empty || current_device(&device, &sms) != cudaSuccess) return 0;
+    return grad_workspace(p, sms);
 }
 
 cudaError_t sm120_launch_score_attention_grad(const SM120ScoreAttentionDesc* desc) {
@@ -117,19 +119,23 @@ cudaError_t sm120_launch_score_attention_grad(const SM120ScoreAttentionDesc* des
     bool empty = false;
     cudaError_t e = resolve(desc, Form::GRADIENT, &p, &empty);
     if (e != cudaSuccess || empty) return e;
-    if (!workspace_ok(desc, grad_workspace(p))) return cudaErrorInvalidValue;
+    // what no device is needed for first: the per-row arrays are the least a workspace holds
+    if (!workspace_ok(desc, row_bytes(p))) return cudaErrorInvalidValue;
     int device = 0, sms = 0;
     e = current_device(&device, &sms);
     if (e != cudaSuccess) return e;
+    if (!workspace_ok(desc, grad_workspace(p, sms))) return cudaErrorInvalidValue;
     p.neg_lse = static_cast<float*>(desc->workspace);
     p.neg_delta = p.neg_lse + stats_bytes(p) / sizeof(float);
     p.ranges = reinterpret_cast<int2*>(p.neg_delta + stats_bytes(p) / sizeof(float));
-    e = sa_grad_prepare_launch(p, desc->stream);
-    if (e != cudaSuccess) return e;
-    const bool tc = sa_tc_grad_supported(p);
-    e = tc ? sa_tc_grad(p, device, desc->stream) : sa_simt_grad(p, desc->stream);
-    if (e == cudaSuccess)
-        note_launches(tc ? (p.head_dim > 64 ? "score_attention_grad_tcgen05_d128" : "score_attention_grad_tcgen05_d64") : "score_attention_grad_simt", 3);
+    if (!sa_tc_grad_supported(p)) {
+        e = sa_simt_grad(p, desc->stream);
+        if (e == cudaSuccess) note_launches("score_attention_grad_simt", 3);
+        return e;
+    }
+    int launches = 0;
+    e = sa_tc_grad(p, static_cast<char*>(desc->workspace) + row_bytes(p), device, sms, desc->stream, &launches);
+    if (e == cudaSuccess) note_launches(p.head_dim > 64 ? "score_attention_grad_tcgen05_d128" : "score_attention_grad_tcgen05_d64", launches);
     return e;
 }
 

@@ -86,12 +86,9 @@ __device__ __forceinline__ void sa_query_range(const ScoreParams& p, int b, int 
     end = max(to, from);
 }
 
-// shared by the two kernel families (score_attention_simt.cu): fills neg_lse, neg_delta and ranges
-cudaError_t sa_grad_prepare_launch(const ScoreParams& p, cudaStream_t stream);
-
 // Plain FFMA kernels: any type, head dimension up to 256, any strides.
 cudaError_t sa_simt_forward(const ScoreParams& p, cudaStream_t stream);
-cudaError_t sa_simt_grad(const ScoreParams& p, cudaStream_t stream);
+cudaError_t sa_simt_grad(const ScoreParams& p, cudaStream_t stream);      // three launches
 cudaError_t sa_simt_decode(const ScoreParams& p, cudaStream_t stream);
 
 // Tensor-core forward (score_attention_tcgen05.cuh): 16-bit types, head dimension a multiple of 8 up to 128, operands that TMA can address.
@@ -102,9 +99,11 @@ cudaError_t sa_tc_forward(const ScoreParams& p, int device, cudaStream_t stream)
 // `parts` parts of `tiles_per_part`, results in part_out / part_lse (score_attention_decode.cu).
 cudaError_t sa_tc_prefix(const ScoreParams& p, int parts, int tiles_per_part, float* part_out, float* part_lse, int device, cudaStream_t stream);
 
-// Tensor-core gradients (score_attention_grad_tcgen05.cuh), after sa_grad_prepare_launch; the same limits.
+// Tensor-core gradients (score_attention_grad_tcgen05.cuh); the same limits.  `workspace` is what sa_tc_grad_workspace asks for behind the
+// three per-row arrays.
 bool sa_tc_grad_supported(const ScoreParams& p);
-cudaError_t sa_tc_grad(const ScoreParams& p, int device, cudaStream_t stream);
+size_t sa_tc_grad_workspace(const ScoreParams& p, int sms);
+cudaError_t sa_tc_grad(const ScoreParams& p, void* workspace, int device, int sms, cudaStream_t stream, int* launches);
 
 // Single-token form for 16-bit types (score_attention_decode.cu): the same limits.
 bool sa_tma_ok(const void* ptr, const int64_t* strides, const int64_t* extents, int count);

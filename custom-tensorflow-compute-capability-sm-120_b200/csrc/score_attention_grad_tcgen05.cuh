@@ -48,6 +48,8 @@ struct SaGradParams {
     ScoreParams s;
     float scale_log2, cap_in, cap_log2, cap_u;           // as in SaFwdParams
     int bf16;
+    int parts;                           // KEYS: the streamed tiles of a block are cut into this many parts, one block each
+    float* part_sums;                    // [part][grad_K, grad_V][batch][kv_heads][seq_k][head_dim], read when parts > 1
     unsigned long long wait_limit_ns;
     unsigned int* status;
 };
@@ -217,7 +219,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const ScoreParams& sp = p.s;
-    // Grid: (batch x row heads, row tiles).  A causal launch starts the long tiles first: the first keys, the last queries.
+    // Grid: (batch x row heads, row tiles, parts).  A causal launch starts the long tiles first: the first keys, the last queries.
     const int row_heads = KEYS ? sp.kv_heads : sp.heads;
     const int b = static_cast<int>(blockIdx.x) / row_heads, rh = static_cast<int>(blockIdx.x) % row_heads;
     const int r0 = static_cast<int>(!KEYS && sp.causal ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * ATT_BM;
@@ -293,15 +295,19 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     const uint32_t tmem_base = *tmem_holder;
     const int u_lo = stream_range[0], u_hi = stream_range[1];
     const int per_head = u_hi > u_lo ? (u_hi - (u_lo & ~3) + SG_T - 1) / SG_T : 0;       // tiles of one head
-    const int n_tiles = KEYS ? per_head * sp.group : per_head;
-    const int head0 = KEYS ? rh * sp.group : kvh;                                        // head of the first streamed tile
+    // this block's tiles: all of them, or one of `parts` even shares (blockIdx.z) of the group's heads x tiles
+    const int64_t all_tiles = KEYS ? static_cast<int64_t>(per_head) * sp.group : per_head;
+    const int first_tile = KEYS ? static_cast<int>(all_tiles * blockIdx.z / p.parts) : 0;
+    const int n_tiles = KEYS ? static_cast<int>(all_tiles * (blockIdx.z + 1) / p.parts) - first_tile : per_head;
+    const int t_first = first_tile > 0 ? first_tile % per_head : 0;                      // tile index inside its head, and head, of the first one
+    const int head0 = KEYS ? rh * sp.group + (first_tile > 0 ? first_tile / per_head : 0) : kvh;
 
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SG_REGS_LOW));
 
     if (warp == 0) {
         // ------------------------------ TMA producer ------------------------------
         int issued = 0;
-        int t = 0, head = head0;
+        int t = t_first, head = head0;
         for (int j = 0; j < n_tiles; ++j) {
             bool w = att_wait(empty + 8 * (j % SG_STAGES), ((j / SG_STAGES) & 1) ^ 1u, wctx, 0x42000000u);
             w = __all_sync(0xFFFFFFFFu, w);
@@ -372,7 +378,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             if (j == n_tiles - 1) umma_commit<1>(sums_done);
         };
         // rows of tile j that lie inside the tensor but outside [u_lo, u_hi) become zeros (behind the tensor TMA has filled in zeros)
-        int clean_t = 0;                                       // tile index inside its head
+        int clean_t = t_first;                                 // tile index inside its head
         auto clean = [&](int j) {
             const int u0 = tile_start(u_lo, clean_t);
             uint8_t* stage = smem + 2 * Cfg::X_BYTES + (j % SG_STAGES) * Cfg::STAGE_BYTES;
@@ -432,7 +438,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             hi = range.y;
             if (BIAS) slope_log2 = __ldg(sp.slopes + rh) * SA_LOG2E;
         }
-        int t = 0, head = head0;
+        int t = t_first, head = head0;
         bool ok = true;
         auto next_tile = [&]() {
             if (++t == per_head) {
@@ -557,7 +563,18 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
 #pragma unroll
                     for (int i = 0; i < CW; ++i) o[i] = 0u;
                 }
-                if (r < rows) {
+                if (KEYS && p.parts > 1) {
+                    if (r < rows) {
+                        float* part = p.part_sums + (((static_cast<int64_t>(blockIdx.z) * 2 + which) * sp.batch + b) * sp.kv_heads + rh) * static_cast<int64_t>(sp.seq_k) * sp.head_dim +
+                                      static_cast<int64_t>(r) * sp.head_dim;
+#pragma unroll
+                        for (int v = 0; v < CW / 4; ++v)
+                            if (col + v * 4 < sp.head_dim)
+                                *reinterpret_cast<float4*>(part + col + v * 4) =
+                                    make_float4(__uint_as_float(o[v * 4]) * factor, __uint_as_float(o[v * 4 + 1]) * factor, __uint_as_float(o[v * 4 + 2]) * factor,
+                                                __uint_as_float(o[v * 4 + 3]) * factor);
+                    }
+                } else if (r < rows) {
 #pragma unroll
                     for (int v = 0; v < CW / 8; ++v) {
                         if (col + v * 8 >= sp.head_dim) continue;     // head_dim is a multiple of 8

@@ -301,14 +301,10 @@ cudaError_t sa_simt_decode(const ScoreParams& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-cudaError_t sa_grad_prepare_launch(const ScoreParams& p, cudaStream_t stream) {
+cudaError_t sa_simt_grad(const ScoreParams& p, cudaStream_t stream) {
 #define SA_K(T) sa_grad_prepare_kernel<T>
     SA_BY_TYPE(SA_K, static_cast<int64_t>(p.batch) * p.heads * p.seq_q_pad);
 #undef SA_K
-    return cudaGetLastError();
-}
-
-cudaError_t sa_simt_grad(const ScoreParams& p, cudaStream_t stream) {
 #define SA_K(T) sa_simt_grad_q_kernel<T>
     SA_BY_TYPE(SA_K, static_cast<int64_t>(p.batch) * p.heads * p.seq_q);
 #undef SA_K
