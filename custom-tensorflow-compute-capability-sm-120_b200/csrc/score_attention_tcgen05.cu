@@ -89,7 +89,7 @@ bool sa_tc_grad_supported(const ScoreParams& p) {
 }
 
 // neg_lse, neg_delta and ranges (see sa_grad_prepare_launch) for rows that 16-byte loads can read: sixteen lanes per row, four rows per
-// half warp in flight.  Bound by HBM: out and grad_out are read once (2 x 16 heads x 2048 x 128 bf16: @@PREP@@).
+// half warp in flight.  Bound by HBM: out and grad_out are read once (16 heads x 8192 x 128 bf16, 67 MB: 18 us under a profiler, cold).
 constexpr int PREP_ROWS = 4;
 template <bool BF16>
 __global__ void __launch_bounds__(256)
