@@ -48,6 +48,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint
         : "memory");
 }
 
+// Tiled TMA store of one 4-D box from shared memory; what lies outside the tensor is clipped
+__device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+        ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(src), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
 // two floats rounded to the 16-bit type and packed, the first in the low half
 __device__ __forceinline__ uint32_t pack16(float a, float b, bool bf16) {
     if (bf16) {

@@ -8,8 +8,8 @@
 
 namespace sm120 {
 
-extern template cudaError_t sa_fwd_launch_d<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaFwdParams&, bool, dim3, int, cudaStream_t);
-extern template cudaError_t sa_fwd_launch_d<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaFwdParams&, bool, dim3, int, cudaStream_t);
+extern template cudaError_t sa_fwd_launch_d<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaFwdParams&, bool, dim3, int, cudaStream_t);
+extern template cudaError_t sa_fwd_launch_d<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaFwdParams&, bool, dim3, int, cudaStream_t);
 
 // 16-byte aligned base, and strides that are positive multiples of 16 bytes below TMA's 2^40 bytes wherever a second element exists
 bool sa_tma_ok(const void* ptr, const int64_t* strides, const int64_t* extents, int count) {
@@ -45,14 +45,15 @@ cudaError_t sa_tc_forward(const ScoreParams& p, int device, cudaStream_t stream)
     SaFwdParams fp{};
     sa_fwd_constants(fp, p, device);
     if (fp.status == nullptr) return cudaErrorInvalidSymbol;
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tk, tv, to;
     const int64_t d = p.head_dim;
     if (!tc_encode_4d(&tq, p.q, p.dtype, {d, p.seq_q, p.heads, p.batch}, {p.q_st[2], p.q_st[1], p.q_st[0]}, {64, ATT_BM, 1, 1}) ||
         !tc_encode_4d(&tk, p.k, p.dtype, {d, p.seq_k, p.kv_heads, p.batch}, {p.k_st[2], p.k_st[1], p.k_st[0]}, {64, ATT_BN, 1, 1}) ||
-        !tc_encode_4d(&tv, p.v, p.dtype, {d, p.seq_k, p.kv_heads, p.batch}, {p.v_st[2], p.v_st[1], p.v_st[0]}, {64, 64, 1, 1}))
+        !tc_encode_4d(&tv, p.v, p.dtype, {d, p.seq_k, p.kv_heads, p.batch}, {p.v_st[2], p.v_st[1], p.v_st[0]}, {64, 64, 1, 1}) ||
+        !tc_encode_4d(&to, p.out, p.dtype, {d, p.seq_q, p.heads, p.batch}, {p.o_st[2], p.o_st[1], p.o_st[0]}, {64, 32, 1, 1}))
         return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(p.batch) * p.heads, (p.seq_q + ATT_BM - 1) / ATT_BM, 1);
-    return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, fp, false, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, fp, false, grid, device, stream);
+    return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, to, fp, false, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, to, fp, false, grid, device, stream);
 }
 
 cudaError_t sa_tc_prefix(const ScoreParams& p, int parts, int tiles_per_part, float* part_out, float* part_lse, int device, cudaStream_t stream) {
@@ -71,7 +72,7 @@ cudaError_t sa_tc_prefix(const ScoreParams& p, int parts, int tiles_per_part, fl
         !tc_encode_4d(&tv, p.prefix_v, p.dtype, {d, p.prefix_len, p.kv_heads, 1}, {p.pv_st[1], p.pv_st[0], 0}, {64, 64, 1, 1}))
         return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(p.kv_heads), (p.batch + fp.batch_per_tile - 1) / fp.batch_per_tile, parts);
-    return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, fp, true, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, fp, true, grid, device, stream);
+    return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, tq, fp, true, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, tq, fp, true, grid, device, stream);
 }
 
 extern template cudaError_t sa_grad_launch_d<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaGradParams&, bool, dim3, int, cudaStream_t);

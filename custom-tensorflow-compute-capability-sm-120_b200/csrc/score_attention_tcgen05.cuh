@@ -11,13 +11,16 @@
 //     a tile tests single keys only when some row's range ends inside it (one vote per warp).
 //   * Scores.  The cap and the distance bias are applied to the 128 scores in registers before the maximum:
 //     tanh(u) as a polynomial on packed FMAs while a row's scores of the tile are within 0.8 caps, else 1 - 2 / (1 + e^2u), two more
-//     MUFU operations a score (ex2, rcp) next to the softmax's one, which then bound the tile (@@CAPTIMES@@); the bias
+//     MUFU operations a score (ex2, rcp) next to the softmax's one, which then bound the tile (16 heads x 8192 x 128: 974 instead
+//     of 727 us; 495 without a cap); the bias
 //     is one packed multiply-add, because on one side of the query it is linear in the key index (the tile across
 //     the diagonal of a bidirectional mask takes the absolute value key by key).  Everything is in log2 units.
 //   * Tensors.  4-D tensor maps take any strides; query head h reads key head h / group.  Columns behind head_dim
 //     are the map's zero fill.
 //   * Keys behind kv_hi in the last tile may hold anything, and P = 0 does not silence a NaN in V: the issuing warp zeroes those
 //     rows of V in shared memory before it uses the tile.
+//   * Output.  Rows go through shared memory (Q's, which is done with) and leave as TMA stores of 32 rows x 64 columns per warp: written by their
+//     threads, 16 bytes a row at a time, they took 3000 to 4000 of a 16-tile block's 38000 cycles (@@STORES@@).
 // TOKEN: the rows are the batch's single-token queries against the prefix that they share, [entry x group head]
 // of one key head as 128-row tiles, so the prefix is read once per 128 rows; the key tiles are cut into
 // parts, and each part writes its normalised fp32 rows and their lse for the join (score_attention_decode.cu).
@@ -173,6 +176,7 @@ __global__ void __launch_bounds__(ATT_THREADS, 1)
 sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
                              const __grid_constant__ CUtensorMap tmap_k,
                              const __grid_constant__ CUtensorMap tmap_v,
+                             const __grid_constant__ CUtensorMap tmap_o,
                              const __grid_constant__ SaFwdParams p) {
     using Cfg = SaCfg<D>;
     constexpr bool MODIFIED = CAP || BIAS;
@@ -259,6 +263,7 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
         prefetch_tmap(&tmap_q);
         prefetch_tmap(&tmap_k);
         prefetch_tmap(&tmap_v);
+        if (!TOKEN) prefetch_tmap(&tmap_o);
         int lo, hi, other;
         if (TOKEN) {
             lo = static_cast<int>(blockIdx.z) * p.tiles_per_part * ATT_BN;
@@ -444,7 +449,7 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
         } else {
             const int q = q0 + row;
             live = q < sp.seq_q;
-            out_row = b * sp.o_st[0] + h * sp.o_st[1] + q * sp.o_st[2];
+            out_row = 0;                                       // the tensor map knows
             lse_row = (static_cast<int64_t>(b) * sp.heads + h) * sp.seq_q + q;
             sa_row_range(sp, b, min(q, sp.seq_q - 1), lo, hi);
             pos = q + first_pos;
@@ -601,25 +606,38 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = 0.0f;
                 }
-                if (live) {
-                    const int col = g * HD + c * 32;            // head_dim is a multiple of 8
-                    if (TOKEN) {
+                const int col = g * HD + c * 32;
+                if (TOKEN) {
+                    if (live) {
 #pragma unroll
                         for (int v = 0; v < 8; ++v)
-                            if (col + v * 4 < sp.head_dim)
+                            if (col + v * 4 < sp.head_dim)              // head_dim is a multiple of 8
                                 *reinterpret_cast<float4*>(p.part_out + out_row + col + v * 4) = make_float4(r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
-                    } else {
-                        uint16_t* dst = static_cast<uint16_t*>(sp.out) + out_row + col;
-#pragma unroll
-                        for (int v = 0; v < 4; ++v)
-                            if (col + v * 8 < sp.head_dim)
-                                *reinterpret_cast<uint4*>(dst + v * 8) =
-                                    make_uint4(pack16(r[v * 8], r[v * 8 + 1], bf16), pack16(r[v * 8 + 2], r[v * 8 + 3], bf16),
-                                               pack16(r[v * 8 + 4], r[v * 8 + 5], bf16), pack16(r[v * 8 + 6], r[v * 8 + 7], bf16));
                     }
+                } else {
+                    // every score product is complete (o_done): Q's place takes the block's rows, in the swizzle of a TMA box
+                    const uint32_t dst = q_smem + (col >> 6) * (ATT_BM * 128) + row * 128;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        st_shared_v4(dst + (((((col & 63) >> 3) + v) ^ (row & 7)) << 4), pack16(r[v * 8], r[v * 8 + 1], bf16),
+                                     pack16(r[v * 8 + 2], r[v * 8 + 3], bf16), pack16(r[v * 8 + 4], r[v * 8 + 5], bf16), pack16(r[v * 8 + 6], r[v * 8 + 7], bf16));
                 }
             }
             tcgen05_fence_before();
+        }
+        if (!TOKEN) {
+            fence_proxy_async_smem();
+            // at D = 64 the two warps of a lane group fill the two halves of the same 128-byte rows; every warp comes here, aborted or not
+            if (D == 64) asm volatile("bar.sync %0, 64;" ::"r"(1 + lane_group) : "memory");
+            else __syncwarp();
+            const int first = q0 + lane_group * 32;
+            if (ok && first < sp.seq_q && (D == 128 || g == 0) && elect_one_sync()) {
+                const int block = D == 128 ? g : 0;             // this warp's 64 columns
+                if (block * 64 < sp.head_dim) tma_store_4d(&tmap_o, q_smem + block * (ATT_BM * 128) + lane_group * (32 * 128), block * 64, first, h, b);
+                bulk_commit_group();
+                bulk_wait_group_read<0>();
+            }
+            __syncwarp();
         }
     }
 
@@ -636,8 +654,8 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
 // One variant's launch.  The register hand-over inside the kernel balances only if the kernel starts with ATT_REGS_LAUNCH
 // registers, so a build that compiled to another count is refused.
 template <int D, bool CAP, bool BIAS, bool TOKEN>
-cudaError_t sa_fwd_variant(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SaFwdParams& p, dim3 grid, int device,
-                           cudaStream_t stream) {
+cudaError_t sa_fwd_variant(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const SaFwdParams& p, dim3 grid,
+                           int device, cudaStream_t stream) {
     static std::atomic<uint64_t> attr_done{0};
     auto kern = sm120_score_attention_kernel<D, CAP, BIAS, TOKEN>;
     const uint64_t bit = 1ull << (device & 63);
@@ -650,26 +668,26 @@ cudaError_t sa_fwd_variant(const CUtensorMap& tq, const CUtensorMap& tk, const C
         if (e != cudaSuccess) return e;
         attr_done.fetch_or(bit, std::memory_order_release);
     }
-    kern<<<grid, ATT_THREADS, SaCfg<D>::SMEM, stream>>>(tq, tk, tv, p);
+    kern<<<grid, ATT_THREADS, SaCfg<D>::SMEM, stream>>>(tq, tk, tv, to, p);
     return cudaGetLastError();
 }
 
 // the variants are compiled in score_attention_tcgen05_d64.cu and _d128.cu
 template <int D>
-cudaError_t sa_fwd_launch_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SaFwdParams& p, bool token, dim3 grid,
-                            int device, cudaStream_t stream);
+cudaError_t sa_fwd_launch_d(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const SaFwdParams& p, bool token,
+                            dim3 grid, int device, cudaStream_t stream);
 
 #define SA_FWD_INSTANTIATE(D)                                                                                                         \
     template <>                                                                                                                       \
-    cudaError_t sa_fwd_launch_d<D>(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SaFwdParams& p,          \
-                                   bool token, dim3 grid, int device, cudaStream_t stream) {                                          \
+    cudaError_t sa_fwd_launch_d<D>(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,        \
+                                   const SaFwdParams& p, bool token, dim3 grid, int device, cudaStream_t stream) {                    \
         const bool cap = p.s.softcap > 0.0f, bias = p.s.slopes != nullptr;                                                            \
         auto pick = [&](auto tok) {                                                                                                   \
             constexpr bool T = decltype(tok)::value;                                                                                  \
-            if (cap) return bias ? sa_fwd_variant<D, true, true, T>(tq, tk, tv, p, grid, device, stream)                              \
-                                 : sa_fwd_variant<D, true, false, T>(tq, tk, tv, p, grid, device, stream);                            \
-            return bias ? sa_fwd_variant<D, false, true, T>(tq, tk, tv, p, grid, device, stream)                                      \
-                        : sa_fwd_variant<D, false, false, T>(tq, tk, tv, p, grid, device, stream);                                    \
+            if (cap) return bias ? sa_fwd_variant<D, true, true, T>(tq, tk, tv, to, p, grid, device, stream)                          \
+                                 : sa_fwd_variant<D, true, false, T>(tq, tk, tv, to, p, grid, device, stream);                        \
+            return bias ? sa_fwd_variant<D, false, true, T>(tq, tk, tv, to, p, grid, device, stream)                                  \
+                        : sa_fwd_variant<D, false, false, T>(tq, tk, tv, to, p, grid, device, stream);                                \
         };                                                                                                                            \
         return token ? pick(std::true_type{}) : pick(std::false_type{});                                                              \
     }
