@@ -196,6 +196,8 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                   const __grid_constant__ CUtensorMap tmap_y,
                                   const __grid_constant__ CUtensorMap tmap_u,
                                   const __grid_constant__ CUtensorMap tmap_w,
+                                  const __grid_constant__ CUtensorMap tmap_g1,
+                                  const __grid_constant__ CUtensorMap tmap_g2,
                                   const __grid_constant__ SaGradParams p) {
     using Cfg = SgCfg<D>;
     constexpr int DB = D / 64;
@@ -541,10 +543,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             tcgen05_fence_after();
 #pragma unroll
             for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
-                void* base = KEYS ? (which == 0 ? sp.grad_k : sp.grad_v) : sp.grad_q;
-                const int64_t* st = KEYS ? (which == 0 ? sp.gk_st : sp.gv_st) : sp.gq_st;
                 const float factor = which == 0 ? sp.scale : 1.0f;
-                uint16_t* dst = static_cast<uint16_t*>(base) + b * st[0] + rh * st[1] + r * st[2];
                 uint32_t o[CW];
                 auto load_sums = [&](uint32_t taddr, uint32_t (&v)[CW]) {
                     if constexpr (CW == 32) tmem_ld_32x32_sync(taddr, v);
@@ -574,19 +573,37 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                                     make_float4(__uint_as_float(o[v * 4]) * factor, __uint_as_float(o[v * 4 + 1]) * factor, __uint_as_float(o[v * 4 + 2]) * factor,
                                                 __uint_as_float(o[v * 4 + 3]) * factor);
                     }
-                } else if (r < rows) {
+                } else {
+                    // every product is complete: X's and Y's places take the block's rows, in the swizzle of a TMA box
+                    const uint32_t dst = (which == 0 ? x_smem : y_smem) + (col >> 6) * (ATT_BM * 128) + row * 128;
 #pragma unroll
                     for (int v = 0; v < CW / 8; ++v) {
-                        if (col + v * 8 >= sp.head_dim) continue;     // head_dim is a multiple of 8
                         uint32_t w[4];
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             w[k] = pack16(__uint_as_float(o[v * 8 + 2 * k]) * factor, __uint_as_float(o[v * 8 + 2 * k + 1]) * factor, p.bf16);
-                        *reinterpret_cast<uint4*>(dst + col + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                        st_shared_v4(dst + (((((col & 63) >> 3) + v) ^ (row & 7)) << 4), w[0], w[1], w[2], w[3]);
                     }
                 }
             }
             tcgen05_fence_before();
+        }
+        if (!KEYS || p.parts == 1) {
+            // the four warps of a lane group hold the columns of the same 32 rows; every warp comes here, aborted or not
+            fence_proxy_async_smem();
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + lane_group) : "memory");
+            const int first = r0 + lane_group * 32;
+            if (ok && first < rows && g == 0 && half == 0 && elect_one_sync()) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    if (d * 64 >= sp.head_dim) continue;
+                    tma_store_4d(&tmap_g1, x_smem + d * (ATT_BM * 128) + lane_group * (32 * 128), d * 64, first, rh, b);
+                    if (KEYS) tma_store_4d(&tmap_g2, y_smem + d * (ATT_BM * 128) + lane_group * (32 * 128), d * 64, first, rh, b);
+                }
+                bulk_commit_group();
+                bulk_wait_group_read<0>();
+            }
+            __syncwarp();
         }
     }
 
@@ -600,9 +617,12 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     }
 }
 
+struct SaGradMaps {
+    CUtensorMap x, y, u, w, g1, g2;      // rows, stream, and the outputs of A1 and (KEYS) A2
+};
+
 template <int D, bool KEYS, bool CAP, bool BIAS>
-cudaError_t sa_grad_variant(const CUtensorMap& tx, const CUtensorMap& ty, const CUtensorMap& tu, const CUtensorMap& tw, const SaGradParams& p,
-                            dim3 grid, int device, cudaStream_t stream) {
+cudaError_t sa_grad_variant(const SaGradMaps& m, const SaGradParams& p, dim3 grid, int device, cudaStream_t stream) {
     static std::atomic<uint64_t> attr_done{0};
     auto kern = sm120_score_attention_grad_kernel<D, KEYS, CAP, BIAS>;
     const uint64_t bit = 1ull << (device & 63);
@@ -616,26 +636,24 @@ cudaError_t sa_grad_variant(const CUtensorMap& tx, const CUtensorMap& ty, const 
         if (e != cudaSuccess) return e;
         attr_done.fetch_or(bit, std::memory_order_release);
     }
-    kern<<<grid, SG_THREADS, SgCfg<D>::SMEM, stream>>>(tx, ty, tu, tw, p);
+    kern<<<grid, SG_THREADS, SgCfg<D>::SMEM, stream>>>(m.x, m.y, m.u, m.w, m.g1, m.g2, p);
     return cudaGetLastError();
 }
 
 // the variants are compiled in score_attention_grad_tcgen05_d64.cu and _d128.cu
 template <int D>
-cudaError_t sa_grad_launch_d(const CUtensorMap& tx, const CUtensorMap& ty, const CUtensorMap& tu, const CUtensorMap& tw, const SaGradParams& p,
-                             bool keys, dim3 grid, int device, cudaStream_t stream);
+cudaError_t sa_grad_launch_d(const SaGradMaps& m, const SaGradParams& p, bool keys, dim3 grid, int device, cudaStream_t stream);
 
 #define SA_GRAD_INSTANTIATE(D)                                                                                                        \
     template <>                                                                                                                       \
-    cudaError_t sa_grad_launch_d<D>(const CUtensorMap& tx, const CUtensorMap& ty, const CUtensorMap& tu, const CUtensorMap& tw,       \
-                                    const SaGradParams& p, bool keys, dim3 grid, int device, cudaStream_t stream) {                   \
+    cudaError_t sa_grad_launch_d<D>(const SaGradMaps& m, const SaGradParams& p, bool keys, dim3 grid, int device, cudaStream_t stream) { \
         const bool cap = p.s.softcap > 0.0f, bias = p.s.slopes != nullptr;                                                            \
         auto pick = [&](auto k) {                                                                                                     \
             constexpr bool K = decltype(k)::value;                                                                                    \
-            if (cap) return bias ? sa_grad_variant<D, K, true, true>(tx, ty, tu, tw, p, grid, device, stream)                         \
-                                 : sa_grad_variant<D, K, true, false>(tx, ty, tu, tw, p, grid, device, stream);                       \
-            return bias ? sa_grad_variant<D, K, false, true>(tx, ty, tu, tw, p, grid, device, stream)                                 \
-                        : sa_grad_variant<D, K, false, false>(tx, ty, tu, tw, p, grid, device, stream);                               \
+            if (cap) return bias ? sa_grad_variant<D, K, true, true>(m, p, grid, device, stream)                                      \
+                                 : sa_grad_variant<D, K, true, false>(m, p, grid, device, stream);                                    \
+            return bias ? sa_grad_variant<D, K, false, true>(m, p, grid, device, stream)                                              \
+                        : sa_grad_variant<D, K, false, false>(m, p, grid, device, stream);                                            \
         };                                                                                                                            \
         return keys ? pick(std::true_type{}) : pick(std::false_type{});                                                               \
     }

@@ -75,8 +75,8 @@ cudaError_t sa_tc_prefix(const ScoreParams& p, int parts, int tiles_per_part, fl
     return d > 64 ? sa_fwd_launch_d<128>(tq, tk, tv, tq, fp, true, grid, device, stream) : sa_fwd_launch_d<64>(tq, tk, tv, tq, fp, true, grid, device, stream);
 }
 
-extern template cudaError_t sa_grad_launch_d<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaGradParams&, bool, dim3, int, cudaStream_t);
-extern template cudaError_t sa_grad_launch_d<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const SaGradParams&, bool, dim3, int, cudaStream_t);
+extern template cudaError_t sa_grad_launch_d<64>(const SaGradMaps&, const SaGradParams&, bool, dim3, int, cudaStream_t);
+extern template cudaError_t sa_grad_launch_d<128>(const SaGradMaps&, const SaGradParams&, bool, dim3, int, cudaStream_t);
 
 bool sa_tc_grad_supported(const ScoreParams& p) {
     if (!sa_tc_types_ok(p) || p.seq_k < 1 || p.seq_q < 1) return false;
@@ -220,19 +220,22 @@ cudaError_t sa_tc_grad(const ScoreParams& p, void* workspace, int device, int sm
     auto encode = [&](CUtensorMap* map, const void* ptr, const int64_t (&st)[3], int64_t seq, int64_t heads, int rows) {
         return tc_encode_4d(map, ptr, p.dtype, {d, seq, heads, p.batch}, {st[2], st[1], st[0]}, {64, rows, 1, 1});
     };
-    CUtensorMap x, y, u, w;
+    SaGradMaps m;
     // queries as rows, then keys as rows
-    if (!encode(&x, p.q, p.q_st, p.seq_q, p.heads, ATT_BM) || !encode(&y, p.grad_out, p.go_st, p.seq_q, p.heads, ATT_BM) ||
-        !encode(&u, p.k, p.k_st, p.seq_k, p.kv_heads, SG_T) || !encode(&w, p.v, p.v_st, p.seq_k, p.kv_heads, SG_T))
+    if (!encode(&m.x, p.q, p.q_st, p.seq_q, p.heads, ATT_BM) || !encode(&m.y, p.grad_out, p.go_st, p.seq_q, p.heads, ATT_BM) ||
+        !encode(&m.u, p.k, p.k_st, p.seq_k, p.kv_heads, SG_T) || !encode(&m.w, p.v, p.v_st, p.seq_k, p.kv_heads, SG_T) ||
+        !encode(&m.g1, p.grad_q, p.gq_st, p.seq_q, p.heads, 32))
         return cudaErrorInvalidValue;
+    m.g2 = m.g1;
     dim3 grid(static_cast<unsigned>(p.batch) * p.heads, (p.seq_q + ATT_BM - 1) / ATT_BM, 1);
-    e = d > 64 ? sa_grad_launch_d<128>(x, y, u, w, gp, false, grid, device, stream) : sa_grad_launch_d<64>(x, y, u, w, gp, false, grid, device, stream);
+    e = d > 64 ? sa_grad_launch_d<128>(m, gp, false, grid, device, stream) : sa_grad_launch_d<64>(m, gp, false, grid, device, stream);
     if (e != cudaSuccess) return e;
-    if (!encode(&x, p.k, p.k_st, p.seq_k, p.kv_heads, ATT_BM) || !encode(&y, p.v, p.v_st, p.seq_k, p.kv_heads, ATT_BM) ||
-        !encode(&u, p.q, p.q_st, p.seq_q, p.heads, SG_T) || !encode(&w, p.grad_out, p.go_st, p.seq_q, p.heads, SG_T))
+    if (!encode(&m.x, p.k, p.k_st, p.seq_k, p.kv_heads, ATT_BM) || !encode(&m.y, p.v, p.v_st, p.seq_k, p.kv_heads, ATT_BM) ||
+        !encode(&m.u, p.q, p.q_st, p.seq_q, p.heads, SG_T) || !encode(&m.w, p.grad_out, p.go_st, p.seq_q, p.heads, SG_T) ||
+        !encode(&m.g1, p.grad_k, p.gk_st, p.seq_k, p.kv_heads, 32) || !encode(&m.g2, p.grad_v, p.gv_st, p.seq_k, p.kv_heads, 32))
         return cudaErrorInvalidValue;
     grid = dim3(static_cast<unsigned>(p.batch) * p.kv_heads, (p.seq_k + ATT_BM - 1) / ATT_BM, gp.parts);
-    e = d > 64 ? sa_grad_launch_d<128>(x, y, u, w, gp, true, grid, device, stream) : sa_grad_launch_d<64>(x, y, u, w, gp, true, grid, device, stream);
+    e = d > 64 ? sa_grad_launch_d<128>(m, gp, true, grid, device, stream) : sa_grad_launch_d<64>(m, gp, true, grid, device, stream);
     *launches = 3;
     if (e != cudaSuccess || gp.parts == 1) return e;
     const int64_t quads = static_cast<int64_t>(p.batch) * p.kv_heads * p.seq_k * (p.head_dim / 4);

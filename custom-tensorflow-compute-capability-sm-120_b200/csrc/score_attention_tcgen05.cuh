@@ -20,7 +20,7 @@
 //   * Keys behind kv_hi in the last tile may hold anything, and P = 0 does not silence a NaN in V: the issuing warp zeroes those
 //     rows of V in shared memory before it uses the tile.
 //   * Output.  Rows go through shared memory (Q's, which is done with) and leave as TMA stores of 32 rows x 64 columns per warp: written by their
-//     threads, 16 bytes a row at a time, they took 3000 to 4000 of a 16-tile block's 38000 cycles (@@STORES@@).
+//     threads, 16 bytes a row at a time, they took 3000 to 4000 of a 16-tile block's 38000 cycles: 4 x 16 heads x 2048 x 128 158 -> 149 us.
 // TOKEN: the rows are the batch's single-token queries against the prefix that they share, [entry x group head]
 // of one key head as 128-row tiles, so the prefix is read once per 128 rows; the key tiles are cut into
 // parts, and each part writes its normalised fp32 rows and their lse for the join (score_attention_decode.cu).
