@@ -7,6 +7,10 @@
 // cluster: the blocks leave their normalised rows and log2 denominators in shared memory and each joins a share of the columns from
 // all of them, in ascending order, in the same launch (1 x 32/8 heads x 700 x 128: 5.9 us and no workspace instead of 5.8 + 5.3 us in two launches).
 // Otherwise they go to the workspace and a second kernel joins them the same way.  A single part writes the result itself.
+// Caches that offer more work than the GPU holds at once are STREAMED: the lengths live on the device, so the blocks (as many as run at
+// once) count the 64-key units of all entries themselves and each takes an even, consecutive share of them, whatever the lengths
+// are.  A share begins and ends inside some (entry, key head); those two pieces go to the block's two slots of the workspace, whole ones are
+// written out at once, and the join finds the slots from the same arithmetic (what it brings: DIRECT_KEYS).
 //
 // Block.  Four warps, each with its own ring of 16-key tiles (K and V rows by 16-byte cp.async, rows behind the
 // valid ones never touched: zero fill), so no barrier orders the loop: three tiles of 8 KB per warp and two blocks per SM keep
@@ -59,6 +63,9 @@ struct DecodeParams {
     float scale_log2, cap_in, cap_log2;
     float* part_out;                          // [part][batch][heads][head_dim]
     float* part_lse;                          // [part][batch][heads], log2 units
+    int stream;                               // > 0: the caches are streamed by this many blocks (own.blocks); own.parts is 1: a whole segment's row
+    float* slot_out;                          // [stream][2][16][head_dim]
+    float* slot_lse;                          // [stream][2][16]
     int direct;                               // one part in all: write the result itself
     int cluster;                              // > 1: this many parts are one cluster and join in it; parts vary fastest over the blocks
     int prefix_tiles;                         // the prefix runs on the tcgen05 kernel, this many key tiles per part (0: it runs here)
@@ -115,8 +122,29 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     lo = pack16(a - ha, b - hb, BF16);
 }
 
+// Units (64 keys) of the entries before `b` and of all of them, times key heads and row tiles.  One warp.
+__device__ __forceinline__ int units_of(const DecodeParams& p, int b) {
+    return (min(max(__ldg(p.s.key_lengths + b), 0), p.s.seq_k) + DEC_STEP - 1) / DEC_STEP;
+}
+__device__ __forceinline__ void count_units(const DecodeParams& p, int b, int lane, int& before, int& all) {
+    before = all = 0;
+    for (int i = lane; i < p.s.batch; i += 32) {
+        const int u = units_of(p, i);
+        all += u;
+        if (i < b) before += u;
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, s);
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, s);
+    }
+    const int each = p.s.kv_heads * p.own.row_tiles;     // the plan keeps all units below 2^31
+    before *= each;
+    all *= each;
+}
+
 template <int D, bool BF16, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(DEC_WARPS * 32, 2)
+__global__ void __launch_bounds__(DEC_WARPS * 32, D > 64 ? 2 : 3)
 sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
     constexpr int CH = D / 8;                            // 16-byte pieces per row
     constexpr uint32_t TILE = DEC_KEYS * D * 2;          // bytes of one K (or V) tile
@@ -130,253 +158,324 @@ sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
     const bool common = idx < p.prefix.blocks;
     if (!common) idx -= p.prefix.blocks;
     const DecodeSide& side = common ? p.prefix : p.own;
-    int part = 0;
-    if (p.cluster > 1) {
-        part = idx % p.cluster;
-        idx /= p.cluster;
-    }
-    const int rt = idx % side.row_tiles;
-    idx /= side.row_tiles;
-    const int kvh = idx % sp.kv_heads;
-    idx /= sp.kv_heads;
-    const int b = common ? 0 : idx % sp.batch;
-    if (p.cluster <= 1) part = common ? idx : idx / sp.batch;
-    const int row0 = rt * DEC_ROWS, n_rows = min(DEC_ROWS, (common ? sp.batch * sp.group : sp.group) - row0);
-    const int total = common ? sp.prefix_len : min(max(__ldg(sp.key_lengths + b), 0), sp.seq_k);
-    const int lo = part * side.part_keys, hi = min(total, lo + side.part_keys);
-    if (lo >= hi && p.cluster <= 1 && !(p.direct && part == 0)) return;      // the join does not read this part
-
-    // query fragments: rows lane / 4 and lane / 4 + 8, columns 2 (lane % 4) + {0, 1, 8, 9} of each K step
-    auto row_entry = [&](int r) { return common ? (row0 + r) / sp.group : b; };
-    auto row_head = [&](int r) { return kvh * sp.group + (common ? (row0 + r) % sp.group : row0 + r); };
-    uint32_t qf[KSTEPS][4];
+    const bool stream = p.stream > 0 && !common;
+    int part = 0, rt, kvh, b;
+    int unit = 0, unit_end = 0, seg_units = 0, seg_at = 0;       // streaming: this block's units, the segment's, and the first one's place in it
+    if (stream) {
+        const int block = idx;
+        int before, all;
+        count_units(p, 0, lane, before, all);
+        const int blocks = min(p.stream, all);           // never more than units: no block between two others is without work
+        if (block >= blocks) return;
+        unit = static_cast<int>(static_cast<int64_t>(all) * block / blocks);
+        unit_end = static_cast<int>(static_cast<int64_t>(all) * (block + 1) / blocks);
+        // the entry that holds the first unit: 32 entries at a time
+        const int each = sp.kv_heads * side.row_tiles;
+        int cum = 0;
+        for (b = 0;; b += 32) {
+            const int u = b + lane < sp.batch ? units_of(p, b + lane) * each : 0;
+            int scan = u;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int r = (lane >> 2) + 8 * half;
-        const bool live = r < n_rows;
-        const uint16_t* q = static_cast<const uint16_t*>(sp.q) + (live ? row_entry(r) * sp.q_st[0] + row_head(r) * sp.q_st[1] : 0);
-#pragma unroll
-        for (int t = 0; t < KSTEPS; ++t)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = t * 16 + c * 8 + (lane & 3) * 2;
-                qf[t][c * 2 + half] = live && col < sp.head_dim ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
+            for (int s = 1; s < 32; s <<= 1) {
+                const int o = __shfl_up_sync(0xFFFFFFFFu, scan, s);
+                if (lane >= s) scan += o;
             }
+            const unsigned behind = __ballot_sync(0xFFFFFFFFu, cum + scan > unit);
+            if (behind != 0u) {
+                const int first = __ffs(behind) - 1;
+                cum += __shfl_sync(0xFFFFFFFFu, scan - u, first);
+                b += first;
+                break;
+            }
+            cum += __shfl_sync(0xFFFFFFFFu, scan, 31);
+        }
+        seg_units = units_of(p, b);
+        const int seg = (unit - cum) / seg_units;
+        seg_at = (unit - cum) % seg_units;
+        kvh = seg / side.row_tiles;
+        rt = seg % side.row_tiles;
+        idx = block;
+    } else {
+        if (p.cluster > 1) {
+            part = idx % p.cluster;
+            idx /= p.cluster;
+        }
+        rt = idx % side.row_tiles;
+        idx /= side.row_tiles;
+        kvh = idx % sp.kv_heads;
+        idx /= sp.kv_heads;
+        b = common ? 0 : idx % sp.batch;
+        if (p.cluster <= 1) part = common ? idx : idx / sp.batch;
     }
-    float slope[2] = {0.0f, 0.0f}, pos[2] = {0.0f, 0.0f};
-    if constexpr (BIAS) {
+    for (;;) {
+        const int row0 = rt * DEC_ROWS, n_rows = min(DEC_ROWS, (common ? sp.batch * sp.group : sp.group) - row0);
+        const int total = common ? sp.prefix_len : min(max(__ldg(sp.key_lengths + b), 0), sp.seq_k);
+        int lo, hi;
+        int slot = -1, taken = 0;                            // streaming: where a piece of a segment goes, its units
+        if (stream) {
+            const int left = seg_units - seg_at;
+            taken = min(left, unit_end - unit);
+            lo = seg_at * DEC_STEP;
+            hi = min(total, lo + taken * DEC_STEP);
+            if (seg_at > 0) slot = 2 * idx;                  // begun by another block
+            else if (taken < left) slot = 2 * idx + 1;       // left to another block
+        } else {
+            lo = part * side.part_keys;
+            hi = min(total, lo + side.part_keys);
+            if (lo >= hi && p.cluster <= 1 && !(p.direct && part == 0)) return;      // the join does not read this part
+        }
+
+        // query fragments: rows lane / 4 and lane / 4 + 8, columns 2 (lane % 4) + {0, 1, 8, 9} of each K step
+        auto row_entry = [&](int r) { return common ? (row0 + r) / sp.group : b; };
+        auto row_head = [&](int r) { return kvh * sp.group + (common ? (row0 + r) % sp.group : row0 + r); };
+        uint32_t qf[KSTEPS][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int r = min((lane >> 2) + 8 * half, n_rows - 1);
-            slope[half] = __ldg(sp.slopes + row_head(r)) * SA_LOG2E;
-            // keys of the cache follow the prefix: both count from the side's own first key here
-            const int len = min(max(__ldg(sp.key_lengths + row_entry(r)), 0), sp.seq_k);
-            pos[half] = static_cast<float>(len - 1 + (common ? sp.prefix_len : 0));
+            const int r = (lane >> 2) + 8 * half;
+            const bool live = r < n_rows;
+            const uint16_t* q = static_cast<const uint16_t*>(sp.q) + (live ? row_entry(r) * sp.q_st[0] + row_head(r) * sp.q_st[1] : 0);
+#pragma unroll
+            for (int t = 0; t < KSTEPS; ++t)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int col = t * 16 + c * 8 + (lane & 3) * 2;
+                    qf[t][c * 2 + half] = live && col < sp.head_dim ? *reinterpret_cast<const uint32_t*>(q + col) : 0u;
+                }
         }
-    }
+        float slope[2] = {0.0f, 0.0f}, pos[2] = {0.0f, 0.0f};
+        if constexpr (BIAS) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = min((lane >> 2) + 8 * half, n_rows - 1);
+                slope[half] = __ldg(sp.slopes + row_head(r)) * SA_LOG2E;
+                // keys of the cache follow the prefix: both count from the side's own first key here
+                const int len = min(max(__ldg(sp.key_lengths + row_entry(r)), 0), sp.seq_k);
+                pos[half] = static_cast<float>(len - 1 + (common ? sp.prefix_len : 0));
+            }
+        }
 
-    const uint32_t ring = smem_u32(smem) + warp * (DEC_STAGES * 2 * TILE);
-    const char* kp = reinterpret_cast<const char*>(static_cast<const uint16_t*>(side.k) + b * side.k_st[0] + kvh * side.k_st[1]);
-    const char* vp = reinterpret_cast<const char*>(static_cast<const uint16_t*>(side.v) + b * side.v_st[0] + kvh * side.v_st[1]);
-    const int64_t k_row = side.k_st[2] * 2, v_row = side.v_st[2] * 2;
-    const int n_tiles = hi > lo ? (hi - lo + DEC_KEYS - 1) / DEC_KEYS : 0;          // of the block; warp w takes w, w + 4, ...
-    auto load = [&](int tile, int stage) {
-        const uint32_t dst = ring + stage * (2 * TILE);
+        const uint32_t ring = smem_u32(smem) + warp * (DEC_STAGES * 2 * TILE);
+        const char* kp = reinterpret_cast<const char*>(static_cast<const uint16_t*>(side.k) + b * side.k_st[0] + kvh * side.k_st[1]);
+        const char* vp = reinterpret_cast<const char*>(static_cast<const uint16_t*>(side.v) + b * side.v_st[0] + kvh * side.v_st[1]);
+        const int64_t k_row = side.k_st[2] * 2, v_row = side.v_st[2] * 2;
+        const int n_tiles = hi > lo ? (hi - lo + DEC_KEYS - 1) / DEC_KEYS : 0;          // of the block; warp w takes w, w + 4, ...
+        auto load = [&](int tile, int stage) {
+            const uint32_t dst = ring + stage * (2 * TILE);
 #pragma unroll
-        for (int i = 0; i < DEC_KEYS * CH / 32; ++i) {
-            const int piece = i * 32 + lane, r = piece / CH, c = piece % CH;
-            const int key = lo + tile * DEC_KEYS + r;
-            const bool valid = key < hi && c * 8 < sp.head_dim;
-            const uint32_t at = r * (D * 2) + ((c ^ (r & 7)) << 4);
-            const int64_t src = valid ? key : 0;
-            cp_async16(dst + at, kp + src * k_row + (valid ? c * 16 : 0), valid);
-            cp_async16(dst + TILE + at, vp + src * v_row + (valid ? c * 16 : 0), valid);
-        }
-    };
-    float o[D / 8][4];
+            for (int i = 0; i < DEC_KEYS * CH / 32; ++i) {
+                const int piece = i * 32 + lane, r = piece / CH, c = piece % CH;
+                const int key = lo + tile * DEC_KEYS + r;
+                const bool valid = key < hi && c * 8 < sp.head_dim;
+                const uint32_t at = r * (D * 2) + ((c ^ (r & 7)) << 4);
+                const int64_t src = valid ? key : 0;
+                cp_async16(dst + at, kp + src * k_row + (valid ? c * 16 : 0), valid);
+                cp_async16(dst + TILE + at, vp + src * v_row + (valid ? c * 16 : 0), valid);
+            }
+        };
+        float o[D / 8][4];
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+        for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f};
+            for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+        float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int st = 0; st < DEC_STAGES - 1; ++st) {
-        if (warp + st * DEC_WARPS < n_tiles) load(warp + st * DEC_WARPS, st);
-        cp_async_commit();
-    }
-    int stage = 0;
-    for (int tile = warp; tile < n_tiles; tile += DEC_WARPS) {
-        {
-            const int ahead = tile + (DEC_STAGES - 1) * DEC_WARPS;
-            const int into = stage == 0 ? DEC_STAGES - 1 : stage - 1;
-            if (ahead < n_tiles) load(ahead, into);
+        for (int st = 0; st < DEC_STAGES - 1; ++st) {
+            if (warp + st * DEC_WARPS < n_tiles) load(warp + st * DEC_WARPS, st);
             cp_async_commit();
         }
-        cp_async_wait<DEC_STAGES - 1>();
-        __syncwarp();
-        const uint32_t ks = ring + stage * (2 * TILE), vs = ks + TILE;
-        // S = Q K^T: matrices (keys 0-7, 8-15) x (K columns 0-7, 8-15 of the step)
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
-        const int kr = (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-        for (int t = 0; t < KSTEPS; ++t) {
-            uint32_t f[4];
-            const int c = t * 2 + ((lane >> 3) & 1);
-            ldmatrix4(ks + kr * (D * 2) + ((c ^ (kr & 7)) << 4), f);
-            mma16<BF16>(s[0], qf[t], f[0], f[1]);
-            mma16<BF16>(s[1], qf[t], f[2], f[3]);
-        }
-        // scores in log2 units; keys behind the part's end count as nothing
-        const int key0 = lo + tile * DEC_KEYS + (lane & 3) * 2;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = key0 + n * 8 + (i & 1);
-                float z = s[n][i];
-                if constexpr (CAP) z = fmaf(att_rcp(att_exp2(z * p.cap_in) + 1.0f), -2.0f * p.cap_log2, p.cap_log2);
-                else z *= p.scale_log2;
-                if constexpr (BIAS) z = fmaf(slope[i >> 1], static_cast<float>(key) - pos[i >> 1], z);
-                s[n][i] = key < hi ? z : -CUDART_INF_F;
+        int stage = 0;
+        for (int tile = warp; tile < n_tiles; tile += DEC_WARPS) {
+            {
+                const int ahead = tile + (DEC_STAGES - 1) * DEC_WARPS;
+                const int into = stage == 0 ? DEC_STAGES - 1 : stage - 1;
+                if (ahead < n_tiles) load(ahead, into);
+                cp_async_commit();
             }
-        uint32_t hi_f[4], lo_f[4];
+            cp_async_wait<DEC_STAGES - 1>();
+            __syncwarp();
+            const uint32_t ks = ring + stage * (2 * TILE), vs = ks + TILE;
+            // S = Q K^T: matrices (keys 0-7, 8-15) x (K columns 0-7, 8-15 of the step)
+            float s[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+            const int kr = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+            for (int t = 0; t < KSTEPS; ++t) {
+                uint32_t f[4];
+                const int c = t * 2 + ((lane >> 3) & 1);
+                ldmatrix4(ks + kr * (D * 2) + ((c ^ (kr & 7)) << 4), f);
+                mma16<BF16>(s[0], qf[t], f[0], f[1]);
+                mma16<BF16>(s[1], qf[t], f[2], f[3]);
+            }
+            // scores in log2 units; keys behind the part's end count as nothing
+            const int key0 = lo + tile * DEC_KEYS + (lane & 3) * 2;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + n * 8 + (i & 1);
+                    float z = s[n][i];
+                    if constexpr (CAP) z = fmaf(att_rcp(att_exp2(z * p.cap_in) + 1.0f), -2.0f * p.cap_log2, p.cap_log2);
+                    else z *= p.scale_log2;
+                    if constexpr (BIAS) z = fmaf(slope[i >> 1], static_cast<float>(key) - pos[i >> 1], z);
+                    s[n][i] = key < hi ? z : -CUDART_INF_F;
+                }
+            uint32_t hi_f[4], lo_f[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float mx = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+                const float m_new = fmaxf(m[half], mx), m_use = m_new == -CUDART_INF_F ? 0.0f : m_new;
+                if (__any_sync(0xFFFFFFFFu, m_new != m[half])) {
+                    const float fade = att_exp2(m[half] - m_use);
+                    l[half] *= fade;
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) {
+                        o[n][2 * half] *= fade;
+                        o[n][2 * half + 1] *= fade;
+                    }
+                    m[half] = m_new;
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float p0 = att_exp2(s[n][2 * half] - m_use), p1 = att_exp2(s[n][2 * half + 1] - m_use);
+                    l[half] += p0 + p1;
+                    split16<BF16>(p0, p1, hi_f[n * 2 + half], lo_f[n * 2 + half]);
+                }
+            }
+            // O += P V: V matrices (keys 0-7, 8-15) x (two blocks of 8 columns), transposed on the way
+            const int vr = (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                uint32_t f[4];
+                const int c = n * 2 + (lane >> 4);
+                ldmatrix4_trans(vs + vr * (D * 2) + ((c ^ (vr & 7)) << 4), f);
+                mma16<BF16>(o[2 * n], hi_f, f[0], f[1]);
+                mma16<BF16>(o[2 * n + 1], hi_f, f[2], f[3]);
+                mma16<BF16>(o[2 * n], lo_f, f[0], f[1]);
+                mma16<BF16>(o[2 * n + 1], lo_f, f[2], f[3]);
+            }
+            __syncwarp();                                    // every lane has read the stage that the next turn's load overwrites
+            if (++stage == DEC_STAGES) stage = 0;
+        }
+        cp_async_wait<0>();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            float mx = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-            const float m_new = fmaxf(m[half], mx), m_use = m_new == -CUDART_INF_F ? 0.0f : m_new;
-            if (__any_sync(0xFFFFFFFFu, m_new != m[half])) {
-                const float fade = att_exp2(m[half] - m_use);
-                l[half] *= fade;
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) {
-                    o[n][2 * half] *= fade;
-                    o[n][2 * half + 1] *= fade;
-                }
-                m[half] = m_new;
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const float p0 = att_exp2(s[n][2 * half] - m_use), p1 = att_exp2(s[n][2 * half + 1] - m_use);
-                l[half] += p0 + p1;
-                split16<BF16>(p0, p1, hi_f[n * 2 + half], lo_f[n * 2 + half]);
-            }
+            l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
+            l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
         }
-        // O += P V: V matrices (keys 0-7, 8-15) x (two blocks of 8 columns), transposed on the way
-        const int vr = (lane & 7) + (((lane >> 3) & 1) << 3);
+        // join the four warps in shared memory (the rings are done): rows of D floats, then {m, l} per warp and row
+        __syncthreads();
+        float* rows = reinterpret_cast<float*>(smem);                                     // [warp][16][D]
+        float2* ml = reinterpret_cast<float2*>(smem + DEC_WARPS * DEC_ROWS * D * 4);      // [warp][16]
 #pragma unroll
-        for (int n = 0; n < D / 16; ++n) {
-            uint32_t f[4];
-            const int c = n * 2 + (lane >> 4);
-            ldmatrix4_trans(vs + vr * (D * 2) + ((c ^ (vr & 7)) << 4), f);
-            mma16<BF16>(o[2 * n], hi_f, f[0], f[1]);
-            mma16<BF16>(o[2 * n + 1], hi_f, f[2], f[3]);
-            mma16<BF16>(o[2 * n], lo_f, f[0], f[1]);
-            mma16<BF16>(o[2 * n + 1], lo_f, f[2], f[3]);
+        for (int half = 0; half < 2; ++half) {
+            const int r = (lane >> 2) + 8 * half;
+            float* dst = rows + (warp * DEC_ROWS + r) * D + (lane & 3) * 2;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+            if ((lane & 3) == 0) ml[warp * DEC_ROWS + r] = make_float2(m[half], l[half]);
         }
-        __syncwarp();                                    // every lane has read the stage that the next turn's load overwrites
-        if (++stage == DEC_STAGES) stage = 0;
-    }
-    cp_async_wait<0>();
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 1);
-        l[half] += __shfl_xor_sync(0xFFFFFFFFu, l[half], 2);
-    }
-    // join the four warps in shared memory (the rings are done): rows of D floats, then {m, l} per warp and row
-    __syncthreads();
-    float* rows = reinterpret_cast<float*>(smem);                                     // [warp][16][D]
-    float2* ml = reinterpret_cast<float2*>(smem + DEC_WARPS * DEC_ROWS * D * 4);      // [warp][16]
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int r = (lane >> 2) + 8 * half;
-        float* dst = rows + (warp * DEC_ROWS + r) * D + (lane & 3) * 2;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
-        if ((lane & 3) == 0) ml[warp * DEC_ROWS + r] = make_float2(m[half], l[half]);
-    }
-    __syncthreads();
-    float* done = reinterpret_cast<float*>(ml + DEC_WARPS * DEC_ROWS);                // [16][D]: this part's rows, and their denominators
-    float* done_lse = done + DEC_ROWS * D;
-    for (int i = threadIdx.x; i < n_rows * (D / 4); i += DEC_WARPS * 32) {
-        const int r = i / (D / 4), col = i % (D / 4) * 4;
-        float top = -CUDART_INF_F;
-#pragma unroll
-        for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, ml[w * DEC_ROWS + r].x);
-        const float base = top == -CUDART_INF_F ? 0.0f : top;
-        float sum = 0.0f;
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < DEC_WARPS; ++w) {
-            const float2 x = ml[w * DEC_ROWS + r];
-            const float f = att_exp2(x.x - base);
-            const float4 y = *reinterpret_cast<const float4*>(rows + (w * DEC_ROWS + r) * D + col);
-            sum = fmaf(f, x.y, sum);
-            acc.x = fmaf(f, y.x, acc.x);
-            acc.y = fmaf(f, y.y, acc.y);
-            acc.z = fmaf(f, y.z, acc.z);
-            acc.w = fmaf(f, y.w, acc.w);
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const float lse = sum == 0.0f ? -CUDART_INF_F : base + log2f(sum);
-        const int e = row_entry(r), h = row_head(r);
-        const int64_t row = static_cast<int64_t>(e) * sp.heads + h;
-        if (p.cluster > 1) {
-            *reinterpret_cast<float4*>(done + r * D + col) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            if (col == 0) done_lse[r] = lse;
-        } else if (p.direct) {
-            if (col < sp.head_dim)
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(sp.out) + e * sp.o_st[0] + h * sp.o_st[1] + col) =
-                    make_uint2(pack16(acc.x * inv, acc.y * inv, BF16), pack16(acc.z * inv, acc.w * inv, BF16));
-            if (col == 0 && sp.lse != nullptr) sp.lse[row] = lse * SA_LN2;
-        } else {
-            const int64_t at = static_cast<int64_t>(side.first_part + part) * sp.batch * sp.heads + row;
-            if (col < sp.head_dim)
-                *reinterpret_cast<float4*>(p.part_out + at * sp.head_dim + col) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            if (col == 0) p.part_lse[at] = lse;
-        }
-    }
-    if (p.cluster > 1) {
-        cluster_arrive();
-        cluster_wait();
-        const uint32_t done_at = smem_u32(done), lse_at = smem_u32(done_lse);
-        for (int i = part * DEC_WARPS * 32 + threadIdx.x; i < n_rows * (D / 4); i += p.cluster * DEC_WARPS * 32) {
+        __syncthreads();
+        float* done = reinterpret_cast<float*>(ml + DEC_WARPS * DEC_ROWS);                // [16][D]: this part's rows, and their denominators
+        float* done_lse = done + DEC_ROWS * D;
+        for (int i = threadIdx.x; i < n_rows * (D / 4); i += DEC_WARPS * 32) {
             const int r = i / (D / 4), col = i % (D / 4) * 4;
-            float lse[8], top = -CUDART_INF_F;
+            float top = -CUDART_INF_F;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                lse[c] = -CUDART_INF_F;
-                if (c < p.cluster) lse[c] = ld_cluster(map_to_cta(lse_at + r * 4, c));
-                top = fmaxf(top, lse[c]);
-            }
+            for (int w = 0; w < DEC_WARPS; ++w) top = fmaxf(top, ml[w * DEC_ROWS + r].x);
             const float base = top == -CUDART_INF_F ? 0.0f : top;
             float sum = 0.0f;
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (c >= p.cluster) continue;
-                const float w = att_exp2(lse[c] - base);
-                const float4 y = ld_cluster4(map_to_cta(done_at + (r * D + col) * 4, c));
-                sum += w;
-                acc.x = fmaf(w, y.x, acc.x);
-                acc.y = fmaf(w, y.y, acc.y);
-                acc.z = fmaf(w, y.z, acc.z);
-                acc.w = fmaf(w, y.w, acc.w);
+            for (int w = 0; w < DEC_WARPS; ++w) {
+                const float2 x = ml[w * DEC_ROWS + r];
+                const float f = att_exp2(x.x - base);
+                const float4 y = *reinterpret_cast<const float4*>(rows + (w * DEC_ROWS + r) * D + col);
+                sum = fmaf(f, x.y, sum);
+                acc.x = fmaf(f, y.x, acc.x);
+                acc.y = fmaf(f, y.y, acc.y);
+                acc.z = fmaf(f, y.z, acc.z);
+                acc.w = fmaf(f, y.w, acc.w);
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float lse = sum == 0.0f ? -CUDART_INF_F : base + log2f(sum);
             const int e = row_entry(r), h = row_head(r);
-            if (col < sp.head_dim)
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(sp.out) + e * sp.o_st[0] + h * sp.o_st[1] + col) =
-                    make_uint2(pack16(acc.x * inv, acc.y * inv, BF16), pack16(acc.z * inv, acc.w * inv, BF16));
-            if (col == 0 && sp.lse != nullptr) sp.lse[static_cast<int64_t>(e) * sp.heads + h] = sum == 0.0f ? -CUDART_INF_F : (base + log2f(sum)) * SA_LN2;
+            const int64_t row = static_cast<int64_t>(e) * sp.heads + h;
+            if (slot >= 0) {
+                const int at = slot * DEC_ROWS + r;
+                if (col < sp.head_dim)
+                    *reinterpret_cast<float4*>(p.slot_out + static_cast<int64_t>(at) * sp.head_dim + col) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                if (col == 0) p.slot_lse[at] = lse;
+            } else if (p.cluster > 1) {
+                *reinterpret_cast<float4*>(done + r * D + col) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                if (col == 0) done_lse[r] = lse;
+            } else if (p.direct) {
+                if (col < sp.head_dim)
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(sp.out) + e * sp.o_st[0] + h * sp.o_st[1] + col) =
+                        make_uint2(pack16(acc.x * inv, acc.y * inv, BF16), pack16(acc.z * inv, acc.w * inv, BF16));
+                if (col == 0 && sp.lse != nullptr) sp.lse[row] = lse * SA_LN2;
+            } else {
+                const int64_t at = static_cast<int64_t>(side.first_part + part) * sp.batch * sp.heads + row;
+                if (col < sp.head_dim)
+                    *reinterpret_cast<float4*>(p.part_out + at * sp.head_dim + col) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                if (col == 0) p.part_lse[at] = lse;
+            }
         }
-        cluster_arrive();                                // no block leaves while another may still read its rows
-        cluster_wait();
+        if (p.cluster > 1) {
+            cluster_arrive();
+            cluster_wait();
+            const uint32_t done_at = smem_u32(done), lse_at = smem_u32(done_lse);
+            for (int i = part * DEC_WARPS * 32 + threadIdx.x; i < n_rows * (D / 4); i += p.cluster * DEC_WARPS * 32) {
+                const int r = i / (D / 4), col = i % (D / 4) * 4;
+                float lse[8], top = -CUDART_INF_F;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    lse[c] = -CUDART_INF_F;
+                    if (c < p.cluster) lse[c] = ld_cluster(map_to_cta(lse_at + r * 4, c));
+                    top = fmaxf(top, lse[c]);
+                }
+                const float base = top == -CUDART_INF_F ? 0.0f : top;
+                float sum = 0.0f;
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    if (c >= p.cluster) continue;
+                    const float w = att_exp2(lse[c] - base);
+                    const float4 y = ld_cluster4(map_to_cta(done_at + (r * D + col) * 4, c));
+                    sum += w;
+                    acc.x = fmaf(w, y.x, acc.x);
+                    acc.y = fmaf(w, y.y, acc.y);
+                    acc.z = fmaf(w, y.z, acc.z);
+                    acc.w = fmaf(w, y.w, acc.w);
+                }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const int e = row_entry(r), h = row_head(r);
+                if (col < sp.head_dim)
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(sp.out) + e * sp.o_st[0] + h * sp.o_st[1] + col) =
+                        make_uint2(pack16(acc.x * inv, acc.y * inv, BF16), pack16(acc.z * inv, acc.w * inv, BF16));
+                if (col == 0 && sp.lse != nullptr) sp.lse[static_cast<int64_t>(e) * sp.heads + h] = sum == 0.0f ? -CUDART_INF_F : (base + log2f(sum)) * SA_LN2;
+            }
+            cluster_arrive();                                // no block leaves while another may still read its rows
+            cluster_wait();
+        }
+        if (!stream) break;
+        unit += taken;
+        if (unit >= unit_end) break;
+        // the next segment begins at its first unit: the next row tile, key head, or entry that has keys
+        seg_at = 0;
+        if (++rt == side.row_tiles) {
+            rt = 0;
+            if (++kvh == sp.kv_heads) {
+                kvh = 0;
+                do seg_units = units_of(p, ++b);             // there is one: units are left
+                while (seg_units == 0);
+            }
+        }
+        __syncthreads();                                     // the join's rows lie where the next loads go
     }
 }
 
@@ -395,10 +494,35 @@ sm120_score_decode_join_kernel(const __grid_constant__ DecodeParams p) {
     const int e = static_cast<int>(row / sp.heads), h = static_cast<int>(row % sp.heads);
     const int len = min(max(__ldg(sp.key_lengths + e), 0), sp.seq_k);
     // the parts that were written: all of the prefix's, and the cache's up to the entry's length
-    const int own_parts = p.own.parts > 0 ? (len + p.own.part_keys - 1) / p.own.part_keys : 0;
+    int own_parts = p.own.parts > 0 ? (len + p.own.part_keys - 1) / p.own.part_keys : 0;
+    int64_t slot = -1;                                   // streamed: the first piece's row among the slots; the others' are in the next blocks' slots 0
+    if (p.stream > 0) {
+        own_parts = 0;
+        if (len > 0) {
+            int begin, units;
+            count_units(p, e, lane, begin, units);
+            const int mine = units_of(p, e);
+            const int hg = h % sp.group;
+            begin += (h / sp.group * p.own.row_tiles + hg / DEC_ROWS) * mine;
+            // block c of n holds the units from floor(units c / n)
+            const int blocks = min(p.stream, units);
+            const int64_t first = (static_cast<int64_t>(begin + 1) * blocks - 1) / units, last = (static_cast<int64_t>(begin + mine) * blocks - 1) / units;
+            own_parts = static_cast<int>(last - first) + 1;
+            if (own_parts > 1) slot = (2 * first + 1) * DEC_ROWS + hg % DEC_ROWS;
+            else if (p.prefix.parts == 0) return;        // one block had all of it and wrote the result
+        }
+    }
     const int parts = p.prefix.parts + own_parts;
+    // Part i's denominator and row: pieces of a streamed segment lie in slot 1 of the first block and slot 0 of the following ones.  Selected
+    // by address, not by branch: the loads of several parts stay in flight together.
+    auto in_slot = [&](int i) { return slot >= 0 && i >= p.prefix.parts; };
+    auto row_of = [&](int i) {
+        const int k = i - p.prefix.parts;
+        return in_slot(i) ? slot + (k > 0 ? (2 * k - 1) * DEC_ROWS : 0) : i * all + row;
+    };
+    auto lse_of = [&](int i) { return (in_slot(i) ? p.slot_lse : p.part_lse)[row_of(i)]; };
     float top = -CUDART_INF_F;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_lse[i * all + row]);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse_of(i));
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
     const float base = top == -CUDART_INF_F ? 0.0f : top;
@@ -408,8 +532,9 @@ sm120_score_decode_join_kernel(const __grid_constant__ DecodeParams p) {
     const bool mine = col < sp.head_dim;
 #pragma unroll 4
     for (int i = w0; i < parts; i += WARPS) {
-        const float w = att_exp2(p.part_lse[i * all + row] - base);
-        const float4 y = *reinterpret_cast<const float4*>(p.part_out + (i * all + row) * sp.head_dim + (mine ? col : 0));
+        const float w = att_exp2(lse_of(i) - base);
+        const float* from = (in_slot(i) ? p.slot_out : p.part_out) + row_of(i) * sp.head_dim;
+        const float4 y = *reinterpret_cast<const float4*>(from + (mine ? col : 0));
         sum += w;
         acc.x = fmaf(w, y.x, acc.x);
         acc.y = fmaf(w, y.y, acc.y);
@@ -441,6 +566,9 @@ sm120_score_decode_join_kernel(const __grid_constant__ DecodeParams p) {
 // How a call is cut.  A part is at least one turn of a block (64 keys) and at most PART_KEYS: long caches of ragged length then
 // balance by themselves, and the workspace's traffic stays below 2 / PART_KEYS of the cache's per query row.
 constexpr int64_t PART_KEYS = 1024;
+// Caches longer than this are streamed.  Measured, us (a block per segment or 1024-key parts / streamed): 64 x 8 key heads x 128, half-ragged
+// lengths up to 512: 22.2 / 29.6, 1024: 49 / 44, 2048: 84 / 76, 4096: 144 / 134; 16 x 16 x 64: 512: 8.3 / 14.3, 4096: 48 / 39
+constexpr int64_t DIRECT_KEYS = 768;
 struct DecodePlan {
     DecodeParams p;
     int64_t parts;
@@ -518,10 +646,28 @@ static bool make_plan(const ScoreParams& p, int sms, DecodePlan* plan) {
             return true;
         }
     }
+    // more units than blocks that run at once: stream long caches, and without a prefix give short ones a block per segment, which needs no join
+    const int64_t base = static_cast<int64_t>(dp.own.row_tiles) * p.kv_heads * p.batch;
+    const int64_t units = base * ((p.seq_k + DEC_STEP - 1) / DEC_STEP);
+    if (p.seq_k > 0 && units > fill && units < (1ll << 31) && p.seq_k > DIRECT_KEYS) {
+        dp.stream = static_cast<int>((p.head_dim > 64 ? 2 : 3) * sms);          // registers: two blocks per SM at 128, three at 64
+        dp.own.blocks = dp.stream;
+        dp.own.parts = p.prefix_len > 0 ? 1 : 0;                                // whole segments wait for the prefix in a part of their own
+        dp.own.part_keys = DEC_STEP;
+    } else if (p.seq_k > 0 && p.prefix_len == 0 && base >= fill) {
+        dp.own.parts = 1;
+        dp.own.part_keys = (p.seq_k + DEC_STEP - 1) / DEC_STEP * DEC_STEP;
+        dp.own.blocks = static_cast<int>(base);
+    }
     plan->parts = static_cast<int64_t>(dp.prefix.parts) + dp.own.parts;
-    dp.direct = plan->parts == 1 && dp.prefix_tiles == 0;
+    dp.direct = plan->parts <= 1 && dp.prefix_tiles == 0 && (dp.stream == 0 || p.prefix_len == 0);
     return static_cast<int64_t>(dp.prefix.blocks) + dp.own.blocks < (1ll << 31) && static_cast<int64_t>(p.batch) * p.heads < (1ll << 31);
 }
+
+// workspace: parts' rows, slots' rows, parts' denominators, slots' denominators
+static size_t part_rows(const DecodePlan& plan) { return plan.p.direct && plan.p.stream == 0 ? 0 : static_cast<size_t>(plan.parts) * plan.p.s.batch * plan.p.s.heads; }
+static size_t slot_rows(const DecodePlan& plan) { return static_cast<size_t>(plan.p.stream) * 2 * DEC_ROWS; }
+static size_t plan_floats(const DecodePlan& plan) { return (part_rows(plan) + slot_rows(plan)) * (plan.p.s.head_dim + 1); }
 
 bool sa_tc_decode_supported(const ScoreParams& p) {
     if (!sa_tc_types_ok(p) || (p.seq_k < 1 && p.prefix_len < 1)) return false;
@@ -533,8 +679,8 @@ bool sa_tc_decode_supported(const ScoreParams& p) {
 
 size_t sa_tc_decode_workspace(const ScoreParams& p, int sms) {
     DecodePlan plan;
-    if (!make_plan(p, sms, &plan) || plan.p.direct) return 0;
-    return static_cast<size_t>(plan.parts) * p.batch * p.heads * (p.head_dim + 1) * sizeof(float);
+    if (!make_plan(p, sms, &plan)) return 0;
+    return plan_floats(plan) * sizeof(float);
 }
 
 template <int D, bool BF16>
@@ -576,7 +722,9 @@ cudaError_t sa_tc_decode(const ScoreParams& p, void* workspace, int device, int 
     if (!make_plan(p, sms, &plan)) return cudaErrorInvalidValue;
     DecodeParams& dp = plan.p;
     dp.part_out = static_cast<float*>(workspace);
-    dp.part_lse = dp.part_out + plan.parts * p.batch * p.heads * p.head_dim;
+    dp.slot_out = dp.part_out + part_rows(plan) * p.head_dim;
+    dp.part_lse = dp.slot_out + slot_rows(plan) * p.head_dim;
+    dp.slot_lse = dp.part_lse + part_rows(plan);
     const bool bf16 = p.dtype == SM120_DTYPE_BFLOAT16;
     *launches = 0;
     cudaError_t e = cudaSuccess;
@@ -591,9 +739,10 @@ cudaError_t sa_tc_decode(const ScoreParams& p, void* workspace, int device, int 
         if (e != cudaSuccess) return e;
         ++*launches;
     }
-    if (dp.direct) return e;
+    if (dp.direct && dp.stream == 0) return e;
     const unsigned rows = static_cast<unsigned>(p.batch) * p.heads;
-    if (plan.parts > JOIN_WARP_PARTS) {
+    const int64_t segments = static_cast<int64_t>(dp.own.row_tiles) * p.kv_heads * p.batch;
+    if (plan.parts + dp.stream / segments > JOIN_WARP_PARTS) {
         if (bf16) sm120_score_decode_join_kernel<true, 4><<<rows, 128, 0, stream>>>(dp);
         else sm120_score_decode_join_kernel<false, 4><<<rows, 128, 0, stream>>>(dp);
     } else {
