@@ -360,6 +360,55 @@ def test_tokens_behind_a_shared_prefix(ops, dtype, prefix, case):
     token_and_check(ops, gen, DT[dtype], b, h, hk, s, d, lengths, prefix, softcap, alibi, layout, factor=3.0 if softcap else 1.0)
 
 
+STREAMED = [
+    # b, h, hk, cache rows, d, lengths: more 64-key units than blocks, in every kind of raggedness
+    (3, 32, 8, 4100, 128, lambda e: [4100, 0, 1][e % 3]),
+    (70, 8, 4, 900, 64, lambda e: (e * 37) % 901),
+    (40, 40, 2, 1300, 128, lambda e: 1300 if e == 39 else 0),          # all work in the last entry, two row tiles
+    (9, 4, 4, 5000, 96, lambda e: [64, 63, 65, 128, 5000, 4999, 0, 2, 777][e]),
+    (33, 16, 16, 800, 64, lambda e: 1),                                # fewer units than blocks
+    (34, 8, 8, 1000, 128, lambda e: 0),                                # no work at all
+]
+
+
+@pytest.mark.parametrize("prefix", [0, 70, 6000])
+@pytest.mark.parametrize("case", STREAMED, ids=lambda c: "-".join(map(str, c[:5])))
+def test_streamed_caches(ops, case, prefix):
+    b, h, hk, s, d, length = case
+    gen = torch.Generator(device="cuda").manual_seed(50 + s)
+    token_and_check(ops, gen, torch.bfloat16, b, h, hk, s, d, [length(e) for e in range(b)], prefix, None, prefix == 0)
+
+
+def test_which_kernel_runs(ops, binding):
+    """16-bit tensors run on the tensor cores in every form; nothing falls back unseen."""
+    for d, dtype in ((64, torch.float16), (128, torch.bfloat16), (80, torch.bfloat16)):
+        q, k = torch.randn(1, 4, 130, d, device="cuda").to(dtype), torch.randn(1, 2, 130, d, device="cuda").to(dtype)
+        size = "d128" if d > 64 else "d64"
+        out, lse = ops.score_attention(q, k, k, causal_mask=True, softcap=30.0, return_lse=True)
+        assert binding.last_kernel_name() == f"score_attention_tcgen05_{size}"
+        ops.score_attention_grad(out, q, k, k, out, lse, causal_mask=True, softcap=30.0)
+        assert binding.last_kernel_name() == f"score_attention_grad_tcgen05_{size}"
+        n = torch.tensor([130], dtype=torch.int32, device="cuda")
+        ops.score_attention_decode(q[:, :, 0], k, k, n)
+        assert binding.last_kernel_name() == f"score_attention_decode_{size}"
+        before = binding.launch_count()
+        big = torch.randn(64, 8, d, device="cuda").to(dtype)
+        cache = torch.randn(64, 2, 20, d, device="cuda").to(dtype)
+        common = torch.randn(2, 40000, d, device="cuda").to(dtype)
+        ops.shared_prefix_attention(big, common, common, cache, cache, torch.full((64,), 20, dtype=torch.int32, device="cuda"))
+        assert binding.launch_count() == before + 3                    # prefix on the tcgen05 kernel, caches, join
+    ops.score_attention(q.float(), k.float(), k.float())
+    assert binding.last_kernel_name() == "score_attention_simt"
+
+
+def test_split_gradient_streams(ops):
+    """Few key tiles that many query heads share: the key blocks' streams are cut into parts, of one head or of several."""
+    gen = torch.Generator(device="cuda").manual_seed(60)
+    for b, h, hk, s, d, kind in ((1, 16, 1, 700, 128, "causal"), (1, 2, 2, 3000, 64, "causal"), (2, 6, 1, 900, 96, "documents_causal"),
+                                 (1, 8, 2, 1100, 128, "prefix")):
+        train_and_check(ops, gen, torch.bfloat16, b, h, hk, s, s, d, kind, None, d == 64)
+
+
 @pytest.mark.parametrize("prefix", [300, 5000])
 def test_large_batches_behind_a_shared_prefix(ops, prefix):
     gen = torch.Generator(device="cuda").manual_seed(40)
