@@ -11,6 +11,9 @@ namespace {
 constexpr int64_t INT31 = (1ll << 31) - 1;
 constexpr int64_t MAX_ROWS = 1ll << 32;       // rows of one launch (four to a block of the plain kernels)
 
+// written tensors: no two elements may share an address through a stride of 0
+bool distinct(const int64_t (&st)[3], int64_t a, int64_t b, int64_t c) { return (a <= 1 || st[0] > 0) && (b <= 1 || st[1] > 0) && (c <= 1 || st[2] > 0); }
+
 enum class Form { FORWARD, GRADIENT, TOKEN };
 
 // Checks what can be checked without a device and fills `p`.  *empty: nothing to compute.
@@ -45,6 +48,13 @@ cudaError_t resolve(const SM120ScoreAttentionDesc* d, Form form, ScoreParams* p,
     if (form == Form::GRADIENT) {
         if (d->seq_q > 0 && (d->lse == nullptr || d->grad_out == nullptr || d->grad_q == nullptr)) return cudaErrorInvalidValue;
         if (d->seq_k > 0 && (d->grad_k == nullptr || d->grad_v == nullptr)) return cudaErrorInvalidValue;
+    }
+    if (form == Form::GRADIENT) {
+        if (!distinct(d->grad_q_stride, d->batch, d->heads, d->seq_q) || !distinct(d->grad_k_stride, d->batch, d->kv_heads, d->seq_k) ||
+            !distinct(d->grad_v_stride, d->batch, d->kv_heads, d->seq_k))
+            return cudaErrorInvalidValue;
+    } else if (!distinct(d->out_stride, d->batch, d->heads, d->seq_q)) {
+        return cudaErrorInvalidValue;
     }
     p->batch = static_cast<int>(d->batch); p->heads = static_cast<int>(d->heads); p->kv_heads = static_cast<int>(d->kv_heads);
     p->group = p->heads / p->kv_heads;

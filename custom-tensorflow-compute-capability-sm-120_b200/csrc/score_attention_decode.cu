@@ -172,7 +172,7 @@ sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
         // the entry that holds the first unit: 32 entries at a time
         const int each = sp.kv_heads * side.row_tiles;
         int cum = 0;
-        for (b = 0;; b += 32) {
+        for (b = 0; b < sp.batch; b += 32) {
             const int u = b + lane < sp.batch ? units_of(p, b + lane) * each : 0;
             int scan = u;
 #pragma unroll
@@ -189,7 +189,9 @@ sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
             }
             cum += __shfl_sync(0xFFFFFFFFu, scan, 31);
         }
-        seg_units = units_of(p, b);
+        // (lengths that another stream rewrites meanwhile give a wrong result, but no entry behind the last and no endless walk)
+        seg_units = b < sp.batch ? units_of(p, b) : 0;
+        if (seg_units == 0) return;
         const int seg = (unit - cum) / seg_units;
         seg_at = (unit - cum) % seg_units;
         kvh = seg / side.row_tiles;
@@ -471,8 +473,9 @@ sm120_score_decode_kernel(const __grid_constant__ DecodeParams p) {
             rt = 0;
             if (++kvh == sp.kv_heads) {
                 kvh = 0;
-                do seg_units = units_of(p, ++b);             // there is one: units are left
-                while (seg_units == 0);
+                seg_units = 0;
+                while (seg_units == 0 && ++b < sp.batch) seg_units = units_of(p, b);
+                if (seg_units == 0) break;                   // not reached: units are left
             }
         }
         __syncthreads();                                     // the join's rows lie where the next loads go

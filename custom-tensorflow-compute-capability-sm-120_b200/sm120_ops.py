@@ -917,6 +917,8 @@ def _score_out(out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor
     _check_same("out", out, query)
     if out.shape != query.shape or (out.shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError(f"`out` must have shape {tuple(query.shape)} and a contiguous head dimension")
+    if any(st == 0 and e > 1 for st, e in zip(out.stride(), out.shape)):
+        raise ValueError("`out` must not be an expanded tensor")
     return out
 
 
@@ -992,8 +994,8 @@ def score_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     A query that sees no key gets zeros.  The three integer and slope tensors stay on the
     device: their values are not checked on the host.  ``return_lse`` adds the float32
     [B, H, Sq] logarithm of the softmax denominators (-inf where no key is seen), which
-    ``score_attention_grad`` needs.  ``out`` receives the result.  The call itself is not
-    recorded by autograd (``score_attention_trainable`` is).
+    ``score_attention_grad`` needs.  ``out`` receives the result; it must not overlap the
+    operands.  The call itself is not recorded by autograd (``score_attention_trainable`` is).
 
     float16 / bfloat16 with D a multiple of 8 up to 128 run on the tensor cores; float32 and
     other D up to 256 on a plain kernel."""
@@ -1014,7 +1016,9 @@ def score_attention_grad(grad_out: torch.Tensor, query: torch.Tensor, key: torch
     """Gradients (query, key, value) of ``score_attention`` called with the same operands and
     options, from its result `out`, its `lse` and the result's gradient
     (``sm120_launch_score_attention_grad``).  Key and value gradients are summed over the query
-    heads that share a key head, in a fixed order.  The slopes have no gradient."""
+    heads that share a key head, in a fixed order.  The slopes have no gradient.  Where few or uneven key
+    tiles would leave the GPU idle, the key and value gradients are formed in up to 8 parts: fp32
+    scratch of that many copies comes from torch's allocator for the call."""
     if grad_out is None:
         raise TypeError("grad_out must be a tensor")
     query, key, value, head, side = _score_sequence(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths,

@@ -417,7 +417,13 @@ cudaError_t sm120_launch_attention_ex(
  * strides (and a group of at most 128 heads in the prefix form) run on the tensor
  * cores; everything else, FLOAT32 included, runs on a plain FFMA kernel.
  * Statistics and sums are fp32; the tensor-core kernels round the probabilities
- * (and their gradients) to the inputs' type between the two products.
+ * (and their gradients) to the inputs' type between the two products, so a
+ * FLOAT16 P (dP - D) beyond 65504 overflows as a result would.
+ * Limits: batch and heads up to 65535, lengths up to 2^29, batch x heads x (seq_q + 192)
+ * and batch x kv_heads x seq_k up to 2^32.  Outputs must not overlap the inputs
+ * or themselves (a stride of 0 over more than one element is rejected).  Rows of k and v
+ * (q and grad_out in the gradient) that any row of the entry uses must be finite:
+ * rows that do not see them may still multiply them by a probability of 0.
  */
 typedef struct SM120ScoreAttentionDesc {
     uint32_t struct_size;      /* sizeof(SM120ScoreAttentionDesc); checked */

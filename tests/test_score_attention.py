@@ -195,6 +195,12 @@ def test_c_entry_points_refuse_what_belongs_to_another_form(binding):
         d = _good(binding, form)
         setattr(d, field, value)
         assert getattr(lib, LAUNCH[form])(ctypes.byref(d)) == 1, (form, field)
+    for form, field in (("forward", "out_stride"), ("decode", "out_stride"), ("grad", "grad_q_stride"), ("grad", "grad_k_stride"), ("grad", "grad_v_stride")):
+        d = _good(binding, form)
+        for name in ("out_stride", "grad_q_stride", "grad_k_stride", "grad_v_stride"):
+            getattr(d, name)[:] = (65536, 8192, 64)
+        getattr(d, field)[1] = 0                                                # heads written over one another
+        assert getattr(lib, LAUNCH[form])(ctypes.byref(d)) == 1, (form, field)
     assert lib.sm120_launch_score_attention(None) == 1
     d = _good(binding, "forward")
     d.batch = 0
