@@ -116,22 +116,33 @@ __device__ __forceinline__ float sa_modify_small(uint32_t (&s)[ATT_BN], float ca
     return top;
 }
 
+// Keys outside [start, limit) of the tile become -inf in log2 units, whatever they were.  FACTOR multiplies the others into log2 units (raw
+// products: the caller then goes on with factor 1).  The lower bound is looked at only where a document begins inside the tile.
+template <bool FACTOR>
+__device__ __forceinline__ void sa_mask(uint32_t (&s)[ATT_BN], float factor, int start, int limit) {
+#pragma unroll
+    for (int i = 0; i < ATT_BN; ++i) {
+        const float x = FACTOR ? __uint_as_float(s[i]) * factor : __uint_as_float(s[i]);
+        s[i] = __float_as_uint(i < limit ? x : -CUDART_INF_F);
+    }
+    if (__any_sync(0xFFFFFFFFu, start > 0)) {
+#pragma unroll
+        for (int i = 0; i < ATT_BN; ++i)
+            if (i < start) s[i] = __float_as_uint(-CUDART_INF_F);
+    }
+}
+
 // p = exp2(s * scale2 + neg_m2) (MODIFIED scores already carry the scale) for KEYS keys, packed as 16-bit pairs, added to the
-// partial row sums.  EDGE: only keys with first_off + i < width (unsigned: behind the range's start as well) count.  The sum adds
-// the unrounded exponentials: rounding each first changes it by a relative 2^-9 / sqrt(keys), far inside the output's rounding.
-template <int KEYS, bool EDGE, bool MODIFIED>
-__device__ __forceinline__ void sa_exp_pack(const uint32_t (&s)[KEYS], uint32_t (&packed)[KEYS / 2], uint64_t scale2, uint64_t neg_m2,
-                                            uint64_t& l2, uint32_t first_off, uint32_t width, bool bf16) {
+// partial row sums.  The sum adds the unrounded exponentials: rounding each first changes it by a relative 2^-9 / sqrt(keys), far
+// inside the output's rounding.
+template <int KEYS, bool MODIFIED>
+__device__ __forceinline__ void sa_exp_pack(const uint32_t (&s)[KEYS], uint32_t (&packed)[KEYS / 2], uint64_t scale2, uint64_t neg_m2, uint64_t& l2, bool bf16) {
 #pragma unroll
     for (int i = 0; i < KEYS; i += 2) {
         const uint64_t x = f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         float x0, x1;
         f32x2_split(MODIFIED ? add2(x, neg_m2) : fma2(x, scale2, neg_m2), x0, x1);
-        float p0 = att_exp2(x0), p1 = att_exp2(x1);
-        if constexpr (EDGE) {
-            if (first_off + i >= width) p0 = 0.0f;
-            if (first_off + i + 1 >= width) p1 = 0.0f;
-        }
+        const float p0 = att_exp2(x0), p1 = att_exp2(x1);
         l2 = add2(l2, f32x2(p0, p1));
         packed[i >> 1] = pack16(p0, p1, bf16);
     }
@@ -459,7 +470,6 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
             // behind a purely causal diagonal everything is masked, whatever its bias
             if (sp.causal && sp.prefix_lengths == nullptr) side_first = side_last = 0x7FFFFFFF;
         }
-        const uint32_t width = static_cast<uint32_t>(hi - lo);
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(lane_group * 32) << 16);
         const uint32_t t_s = t_lane + g * ATT_BN;              // S_j, and P_j in its last 64 cells
         const uint32_t t_o = t_lane + Cfg::TMEM_O + g * D;
@@ -482,7 +492,6 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
             for (int c = 0; c < ATT_BN / 32; ++c) tmem_ld_wait_regs(*reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
             // some of the tile's keys do not count for some row of this warp
             const bool edge = __any_sync(0xFFFFFFFFu, key0 < lo || key0 + ATT_BN > hi);
-            const uint32_t off0 = static_cast<uint32_t>(key0 - lo);          // wraps for keys before the range: larger than any width
             if constexpr (MODIFIED) {
                 const float rel = static_cast<float>(key0 - pos);
                 const bool before = !BIAS || key0 + ATT_BN - 1 <= side_first, mixed = BIAS && !before && key0 < side_last;
@@ -505,16 +514,15 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
                     else sa_modify<false, BIAS, false>(s, scale_log2, p.cap_in, p.cap_log2, sl, rel);
                 }
             }
-            float m_tile;
-            if (!edge) {
-                if constexpr (MODIFIED) m_tile = sa_extreme<false>(s);
-                else m_tile = (scale_log2 >= 0.0f ? sa_extreme<false>(s) : sa_extreme<true>(s)) * scale_log2;
-            } else {
-                m_tile = -CUDART_INF_F;
-#pragma unroll
-                for (int i = 0; i < ATT_BN; ++i)
-                    if (off0 + i < width) m_tile = fmaxf(m_tile, MODIFIED ? __uint_as_float(s[i]) : __uint_as_float(s[i]) * scale_log2);
+            // a tile at the border of some row's range is masked here once; what follows is the same for every tile
+            float factor = MODIFIED ? 1.0f : scale_log2;
+            if (edge) {
+                sa_mask<!MODIFIED>(s, scale_log2, lo - key0, hi - key0);
+                factor = 1.0f;
             }
+            float m_tile;
+            if constexpr (MODIFIED) m_tile = sa_extreme<false>(s);
+            else m_tile = (factor >= 0.0f ? sa_extreme<false>(s) : sa_extreme<true>(s)) * factor;
             if (j < 2) {
                 m_ref = m_tile;                                 // the group's first tile: O_g does not exist yet
             } else {
@@ -537,7 +545,7 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
             }
             const float m_use = m_ref == -CUDART_INF_F ? 0.0f : m_ref;      // a row without any key so far
             // p = exp2(z - m), row sum, P (16-bit pairs) -> cells [64, 128) of the S buffer, whose scores are in registers by now
-            const uint64_t scale2 = f32x2(scale_log2, scale_log2), neg_m2 = f32x2(-m_use, -m_use);
+            const uint64_t scale2 = f32x2(factor, factor), neg_m2 = f32x2(-m_use, -m_use);
             uint64_t l2 = f32x2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -545,8 +553,7 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
                 // written its four MMAs may start
                 uint32_t packed[32];
                 const uint32_t(&sc)[64] = *reinterpret_cast<const uint32_t(*)[64]>(&s[c * 64]);
-                if (edge) sa_exp_pack<64, true, MODIFIED>(sc, packed, scale2, neg_m2, l2, off0 + c * 64, width, bf16);
-                else sa_exp_pack<64, false, MODIFIED>(sc, packed, scale2, neg_m2, l2, 0u, 0u, bf16);
+                sa_exp_pack<64, MODIFIED>(sc, packed, scale2, neg_m2, l2, bf16);
                 tmem_st_32x32(t_s + ATT_BN / 2 + c * 32, packed);
                 tmem_st_wait();
                 tcgen05_fence_before();
