@@ -100,6 +100,14 @@ static uint32_t map_key_hash(const MapKey& k) {
     return static_cast<uint32_t>(h);
 }
 
+// The encoder is a driver call and needs a current context.  A host thread whose first CUDA call this is (an autograd engine's backward
+// thread) has none until the runtime binds the device's; every thread's first map passes here, its table being empty.
+static EncodeTiledFn encode_fn_with_context() {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return nullptr;
+    return get_encode_fn();
+}
+
 // 3-D map over a stored matrix: `inner` contiguous elements per row, `outer`
 // rows `pitch` elements apart, `nbatch` matrices `bstride` elements apart.
 static bool encode_3d(CUtensorMap* map, const void* ptr, int dtype, int64_t inner, int64_t outer, int64_t nbatch,
@@ -117,7 +125,7 @@ static bool encode_3d(CUtensorMap* map, const void* ptr, int dtype, int64_t inne
         g_map_hits.fetch_add(1, std::memory_order_relaxed);
         return true;
     }
-    EncodeTiledFn fn = get_encode_fn();
+    EncodeTiledFn fn = encode_fn_with_context();
     if (fn == nullptr) return false;
     cuuint64_t dims[3] = {key.inner, key.outer, key.nbatch};
     cuuint64_t strides[2] = {key.pitch_bytes, key.bstride_bytes};
@@ -177,7 +185,7 @@ bool tc_encode_4d(CUtensorMap* map, const void* ptr, int dtype, const int64_t (&
         g_map_hits.fetch_add(1, std::memory_order_relaxed);
         return true;
     }
-    EncodeTiledFn fn = get_encode_fn();
+    EncodeTiledFn fn = encode_fn_with_context();
     if (fn == nullptr) return false;
     cuuint64_t d[4], st[3];
     cuuint32_t b[4], estr[4] = {1, 1, 1, 1};

@@ -259,6 +259,33 @@ def test_autograd_form(ops):
         assert abs(want - got) <= 1e-3 * float(grads[which].double().norm() * step.double().norm()), which
 
 
+def test_first_call_of_a_host_thread(ops):
+    """A host thread whose first CUDA call is one of these operators (an autograd backward thread, a server's worker)."""
+    import threading
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q, do = (normal(gen, 1, 2, 100, 64, dtype=torch.float16) for _ in range(2))
+    out, lse = ops.score_attention(q, q, q, return_lse=True)
+    want = ops.score_attention_grad(do, q, q, q, out, lse)
+    a, b = normal(gen, 64, 64, dtype=torch.bfloat16), normal(gen, 64, 64, dtype=torch.bfloat16)
+    product = ops.fused_matmul(a, b)
+    got = {}
+
+    def work(name, call):
+        try:
+            got[name] = call()
+        except Exception as e:                                        # reported below, in the test's own thread
+            got[name] = e
+
+    for name, call in (("grad", lambda: ops.score_attention_grad(do, q, q, q, out, lse)), ("forward", lambda: ops.score_attention(q, q, q)),
+                       ("product", lambda: ops.fused_matmul(a, b))):
+        t = threading.Thread(target=work, args=(name, call))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got["grad"], want))
+    assert torch.equal(got["forward"], out) and torch.equal(got["product"], product)
+
+
 def test_streams_and_graphs(ops):
     """Calls on two side streams at once, and forward + backward captured into two graphs that replay after new inputs were written."""
     gen = torch.Generator(device="cuda").manual_seed(8)
