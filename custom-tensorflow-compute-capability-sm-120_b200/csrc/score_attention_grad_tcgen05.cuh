@@ -11,7 +11,10 @@
 //                 rows (fixed, 128)      streamed (tiles of 64)     S = X U^T     dP = Y W^T     sums in TMEM
 //     KEYS        X = K,  Y = V          U = Q, W = grad_O          S^T           dP^T           A1 += dx^T U,  A2 += P^T W
 //     QUERIES     X = Q,  Y = grad_O     U = K, W = V               S             dP             A1 += dx U,  A2 += P (1 - tanh^2) U
-// QUERIES runs first and makes D exact.  D = <grad_O, O> of the prepare pass carries the rounding of O to 16 bits, which where few keys
+// QUERIES runs first, and each of its blocks prepares its rows: neg_lse, D = <grad_O, O> and the key range, which it writes out for the
+// KEYS launch.  (A pass of its own for them costs the same time on long rows, 18 us of 1420 at 16 heads x 8192 x 128, and one launch more on
+// short ones: a step of 2 x 8 x 257 x 64 took 82 us by itself instead of 78.)
+// It also makes D exact.  <grad_O, O> carries the rounding of O to 16 bits, which where few keys
 // dominate a row is as large as the rest of the error together.  The row's sum of P (dP - D) is what D lacks; it corrects grad_Q through A2
 // (grad_Q = scale (A1 - lack A2), one product more) and goes into neg_delta for the KEYS kernel.  Measured on peaked capped
 // scores (relative error of grad_Q, bf16, against 64 bits, 2 x 16 heads x 2048 causal, cap 30): 2.9e-3 before, 2.4e-3 with it, for 4 % of a training step's time.
@@ -63,8 +66,8 @@ struct SgCfg {
     static constexpr uint32_t STAGE_BYTES = 2 * U_BYTES;
     static constexpr uint32_t STAT_OFF = 2 * X_BYTES + SG_STAGES * STAGE_BYTES;
     static constexpr uint32_t BAR_OFF = STAT_OFF + SG_STAGES * STAT_BYTES;
-    // barriers, what the four threads of a row tell each other (QUERIES)
-    static constexpr size_t SMEM_USED = BAR_OFF + 256 + 4 * ATT_BM * 4 + 1024;
+    // barriers, what the four threads of a row tell each other and the rows' <grad_O, O> (QUERIES)
+    static constexpr size_t SMEM_USED = BAR_OFF + 256 + (4 + 1) * ATT_BM * 4 + 1024;
     // every CTA allocates all 512 TMEM columns, so two CTAs must never share an SM: request more than half of its shared memory
     static constexpr size_t SMEM = SMEM_USED > 118784 ? SMEM_USED : 118784;
     static constexpr uint32_t TMEM_COLS = 512;
@@ -178,6 +181,25 @@ __device__ __forceinline__ void sg_chunk(const uint32_t (&s)[32], const uint32_t
     lack += la + lb;
 }
 
+// sum + the products of two rows' eight 16-bit elements
+__device__ __forceinline__ float sg_dot8(const uint4& x, const uint4& y, bool bf16, float sum) {
+    const uint32_t a[4] = {x.x, x.y, x.z, x.w}, c[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float2 u, v;
+        if (bf16) {
+            u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&a[k]));
+            v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&c[k]));
+        } else {
+            u = __half22float2(*reinterpret_cast<const __half2*>(&a[k]));
+            v = __half22float2(*reinterpret_cast<const __half2*>(&c[k]));
+        }
+        sum = fmaf(u.x, v.x, sum);
+        sum = fmaf(u.y, v.y, sum);
+    }
+    return sum;
+}
+
 // Zeroes rows [r0, r1) of a stream tile's U and W and hands the writes to the async proxy.  One warp; it issues the products that read them.
 template <int D>
 __device__ __forceinline__ void sg_zero_rows(uint8_t* stage, int r0, int r1, int lane) {
@@ -217,6 +239,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     volatile uint32_t* abort_flag = tmem_holder + 1;
     volatile int* stream_range = reinterpret_cast<volatile int*>(tmem_holder + 2);      // first streamed row, end
     float* lacks = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);     // [group, half][ATT_BM]
+    float* dots = lacks + 4 * ATT_BM;                                                    // [ATT_BM]
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -432,12 +455,43 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         int lo = 0, hi = 0;
         float row_lse = 0.0f, row_delta = 0.0f, slope_log2 = 0.0f, lack = 0.0f;
         if (!KEYS) {
-            const int64_t at = (static_cast<int64_t>(b) * sp.heads + rh) * sp.seq_q_pad + min(r, sp.seq_q);      // row seq_q is padding: P = 0
-            row_lse = sp.neg_lse[at];
-            row_delta = sp.neg_delta[at];
-            const int2 range = sp.ranges[static_cast<int64_t>(b) * sp.seq_q_pad + min(r, sp.seq_q - 1)];
-            lo = range.x;
-            hi = range.y;
+            // D of the block's rows: eight rows per warp, sixteen lanes and 16-byte loads per row.  (Each row by the threads that own it: every load
+            // then touches 32 rows, and the 4000 cycles that takes came before a block's first tile.)
+            const uint16_t* o = static_cast<const uint16_t*>(sp.out) + b * sp.o_st[0] + rh * sp.o_st[1];
+            const uint16_t* go = static_cast<const uint16_t*>(sp.grad_out) + b * sp.go_st[0] + rh * sp.go_st[1];
+            const int col0 = (lane & 15) * 8, sub0 = (warp - 4) * 8 + (lane >> 4);
+            uint4 x[4], y[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int i = r0 + sub0 + 2 * n;
+                const bool there = i < sp.seq_q && col0 < sp.head_dim;
+                x[n] = there ? __ldg(reinterpret_cast<const uint4*>(o + i * sp.o_st[2] + col0)) : make_uint4(0u, 0u, 0u, 0u);
+                y[n] = there ? __ldg(reinterpret_cast<const uint4*>(go + i * sp.go_st[2] + col0)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float d = sg_dot8(x[n], y[n], p.bf16, 0.0f);
+#pragma unroll
+                for (int sh = 8; sh > 0; sh >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, sh);
+                if ((lane & 15) == 0) dots[sub0 + 2 * n] = d;
+            }
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            const float dot = dots[row];
+            const int rr = min(r, sp.seq_q - 1);
+            const float lse = r < sp.seq_q ? __ldg(sp.lse + (static_cast<int64_t>(b) * sp.heads + rh) * sp.seq_q + r) : -CUDART_INF_F;
+            const bool none = lse == -CUDART_INF_F;            // behind the last row, or a row that saw no key: P = 0
+            row_lse = none ? -CUDART_INF_F : -lse * SA_LOG2E;
+            row_delta = none ? 0.0f : -dot;
+            sa_row_range(sp, b, rr, lo, hi);
+            if (g == 0 && half == 0) {
+                // rows up to the padded end: the last block writes those behind it as well
+                for (int i = r; i < (r0 + ATT_BM >= sp.seq_q ? sp.seq_q_pad : r + 1); i += ATT_BM) {
+                    const int64_t at = (static_cast<int64_t>(b) * sp.heads + rh) * sp.seq_q_pad + i;
+                    sp.neg_lse[at] = i == r ? row_lse : -CUDART_INF_F;
+                    if (i >= sp.seq_q) sp.neg_delta[at] = 0.0f;                  // the others once they are exact, below
+                    if (rh == 0) sp.ranges[static_cast<int64_t>(b) * sp.seq_q_pad + i] = i < sp.seq_q ? make_int2(lo, hi) : make_int2(0, 0);
+                }
+            }
             if (BIAS) slope_log2 = __ldg(sp.slopes + rh) * SA_LOG2E;
         }
         int t = t_first, head = head0;
@@ -534,7 +588,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             lacks[(g * 2 + half) * ATT_BM + row] = lack;
             asm volatile("bar.sync 1, 512;" ::: "memory");
             lack = (lacks[row] + lacks[ATT_BM + row]) + (lacks[2 * ATT_BM + row] + lacks[3 * ATT_BM + row]);
-            if (ok && g == 0 && half == 0 && r < rows && row_lse != -CUDART_INF_F)
+            if (ok && g == 0 && half == 0 && r < rows)
                 sp.neg_delta[(static_cast<int64_t>(b) * sp.heads + rh) * sp.seq_q_pad + r] = row_delta - lack;
         }
         if (ok) {

@@ -1,8 +1,6 @@
 // Host side of the tensor-core kernels of the score-modified attention: what TMA can address, tensor maps, grids.
 // The device code is in score_attention_tcgen05.cuh and score_attention_grad_tcgen05.cuh.
 
-#include <math_constants.h>
-
 #include "score_attention_grad_tcgen05.cuh"
 #include "score_attention_tcgen05.cuh"
 
@@ -84,64 +82,9 @@ bool sa_tc_grad_supported(const ScoreParams& p) {
     if (!sa_tma_ok(p.q, p.q_st, qe, 3) || !sa_tma_ok(p.grad_out, p.go_st, qe, 3) || !sa_tma_ok(p.grad_q, p.gq_st, qe, 3) ||
         !sa_tma_ok(p.k, p.k_st, ke, 3) || !sa_tma_ok(p.v, p.v_st, ke, 3) || !sa_tma_ok(p.grad_k, p.gk_st, ke, 3) || !sa_tma_ok(p.grad_v, p.gv_st, ke, 3))
         return false;
-    // output rows are written, and out is read by the prepare pass, 16 bytes at a time
+    // D reads out and grad_out 16 bytes at a time
     if (!sa_tma_ok(p.out, p.o_st, qe, 3)) return false;
     return p.seq_q <= 65535 * ATT_BM && p.seq_k <= 65535 * ATT_BM;      // grid limits
-}
-
-// neg_lse, neg_delta and ranges (see sa_grad_prepare_launch) for rows that 16-byte loads can read: sixteen lanes per row, four rows per
-// half warp in flight.  Bound by HBM: out and grad_out are read once (16 heads x 8192 x 128 bf16, 67 MB: 18 us under a profiler, cold).
-constexpr int PREP_ROWS = 4;
-template <bool BF16>
-__global__ void __launch_bounds__(256)
-sm120_score_grad_prepare_kernel(const __grid_constant__ ScoreParams p) {
-    const int sub = threadIdx.x >> 4, lane = threadIdx.x & 15;
-    const int64_t rows = static_cast<int64_t>(p.batch) * p.heads * p.seq_q_pad;
-    const int64_t first = (static_cast<int64_t>(blockIdx.x) * 16 + sub) * PREP_ROWS;     // seq_q_pad is a multiple of PREP_ROWS: one head
-    if (first >= rows) return;                                                           // both halves of a warp: rows is a multiple of 8
-    const int i0 = static_cast<int>(first % p.seq_q_pad);
-    const int64_t bh = first / p.seq_q_pad;
-    const int h = static_cast<int>(bh % p.heads), b = static_cast<int>(bh / p.heads);
-    const uint16_t* o = static_cast<const uint16_t*>(p.out) + b * p.o_st[0] + h * p.o_st[1];
-    const uint16_t* g = static_cast<const uint16_t*>(p.grad_out) + b * p.go_st[0] + h * p.go_st[1];
-    uint4 x[PREP_ROWS], y[PREP_ROWS];
-#pragma unroll
-    for (int n = 0; n < PREP_ROWS; ++n) {
-        const bool live = i0 + n < p.seq_q && lane * 8 < p.head_dim;
-        x[n] = live ? __ldg(reinterpret_cast<const uint4*>(o + (i0 + n) * p.o_st[2] + lane * 8)) : make_uint4(0u, 0u, 0u, 0u);
-        y[n] = live ? __ldg(reinterpret_cast<const uint4*>(g + (i0 + n) * p.go_st[2] + lane * 8)) : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-    for (int n = 0; n < PREP_ROWS; ++n) {
-        const uint32_t a[4] = {x[n].x, x[n].y, x[n].z, x[n].w}, c[4] = {y[n].x, y[n].y, y[n].z, y[n].w};
-        float d = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float2 u, v;
-            if (BF16) {
-                u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&a[k]));
-                v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&c[k]));
-            } else {
-                u = __half22float2(*reinterpret_cast<const __half2*>(&a[k]));
-                v = __half22float2(*reinterpret_cast<const __half2*>(&c[k]));
-            }
-            d = fmaf(u.x, v.x, d);
-            d = fmaf(u.y, v.y, d);
-        }
-#pragma unroll
-        for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, s);
-        if (lane != n) continue;                         // one lane per row writes
-        const int i = i0 + n;
-        const float lse = i < p.seq_q ? p.lse[bh * p.seq_q + i] : -CUDART_INF_F;
-        const bool none = lse == -CUDART_INF_F;          // the row saw no key
-        p.neg_lse[first + n] = none ? -CUDART_INF_F : -lse * SA_LOG2E;
-        p.neg_delta[first + n] = none ? 0.0f : -d;
-        if (h == 0) {
-            int2 range = make_int2(0, 0);
-            if (i < p.seq_q) sa_row_range(p, b, i, range.x, range.y);
-            p.ranges[static_cast<int64_t>(b) * p.seq_q_pad + i] = range;
-        }
-    }
 }
 
 // grad_K and grad_V from the parts, added in ascending order; four columns per thread
@@ -198,12 +141,6 @@ size_t sa_tc_grad_workspace(const ScoreParams& p, int sms) {
 }
 
 cudaError_t sa_tc_grad(const ScoreParams& p, void* workspace, int device, int sms, cudaStream_t stream, int* launches) {
-    const int64_t prep_rows = static_cast<int64_t>(p.batch) * p.heads * p.seq_q_pad;
-    const unsigned prep_blocks = static_cast<unsigned>((prep_rows + 16 * PREP_ROWS - 1) / (16 * PREP_ROWS));
-    if (p.dtype == SM120_DTYPE_BFLOAT16) sm120_score_grad_prepare_kernel<true><<<prep_blocks, 256, 0, stream>>>(p);
-    else sm120_score_grad_prepare_kernel<false><<<prep_blocks, 256, 0, stream>>>(p);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
     SaGradParams gp{};
     gp.parts = grad_parts(p, sms);
     gp.part_sums = static_cast<float*>(workspace);
@@ -228,7 +165,7 @@ cudaError_t sa_tc_grad(const ScoreParams& p, void* workspace, int device, int sm
         return cudaErrorInvalidValue;
     m.g2 = m.g1;
     dim3 grid(static_cast<unsigned>(p.batch) * p.heads, (p.seq_q + ATT_BM - 1) / ATT_BM, 1);
-    e = d > 64 ? sa_grad_launch_d<128>(m, gp, false, grid, device, stream) : sa_grad_launch_d<64>(m, gp, false, grid, device, stream);
+    cudaError_t e = d > 64 ? sa_grad_launch_d<128>(m, gp, false, grid, device, stream) : sa_grad_launch_d<64>(m, gp, false, grid, device, stream);
     if (e != cudaSuccess) return e;
     if (!encode(&m.x, p.k, p.k_st, p.seq_k, p.kv_heads, ATT_BM) || !encode(&m.y, p.v, p.v_st, p.seq_k, p.kv_heads, ATT_BM) ||
         !encode(&m.u, p.q, p.q_st, p.seq_q, p.heads, SG_T) || !encode(&m.w, p.grad_out, p.go_st, p.seq_q, p.heads, SG_T) ||
@@ -236,11 +173,11 @@ cudaError_t sa_tc_grad(const ScoreParams& p, void* workspace, int device, int sm
         return cudaErrorInvalidValue;
     grid = dim3(static_cast<unsigned>(p.batch) * p.kv_heads, (p.seq_k + ATT_BM - 1) / ATT_BM, gp.parts);
     e = d > 64 ? sa_grad_launch_d<128>(m, gp, true, grid, device, stream) : sa_grad_launch_d<64>(m, gp, true, grid, device, stream);
-    *launches = 3;
+    *launches = 2;
     if (e != cudaSuccess || gp.parts == 1) return e;
     const int64_t quads = static_cast<int64_t>(p.batch) * p.kv_heads * p.seq_k * (p.head_dim / 4);
     sm120_score_attention_grad_join_kernel<<<dim3(static_cast<unsigned>((quads + 255) / 256), 2, 1), 256, 0, stream>>>(gp);
-    *launches = 4;
+    *launches = 3;
     return cudaGetLastError();
 }
 
