@@ -27,7 +27,8 @@
 // issuing warp's wait and election cost 150 to 230 cycles of each tile's ~1800, so there is one of them (P and dx handed over in two halves, the
 // first half's sums under the second's arithmetic: 1554 instead of 1402 us at 16 heads x 8192 x 64, the same at head size 128).
 // What bounds it at D = 128 (cycle stamps): the tensor pipe.  A tile's sums take 8 x 64 cycles, its scores 16 x 80: an MMA whose A operand comes
-// from shared memory pays 64 cycles for its 4 KB whatever N is, and TMEM has no room for X and Y beside double-buffered scores.
+// from shared memory pays 64 cycles for its 4 KB whatever N is, and TMEM has no room for X and Y beside double-buffered scores.  At D = 64 there is: the rows go
+// there once and the scores read them as the sums read P (16 heads x 8192 x 64: 1390 to 1430 -> 1275 us).
 // TMEM at D = 128: 2 x (64 + 64) scores and dP, 128 + 128 sums = 512 columns: no room for 128-row stream tiles.
 // What a row of the stream needs (neg_lse, neg_delta, its key range) comes with the tile in the KEYS kernel and sits in
 // registers in the other.
@@ -73,8 +74,11 @@ struct SgCfg {
     static constexpr uint32_t TMEM_COLS = 512;
     // S_0, dP_0, S_1, dP_1, each SG_T columns; A1; A2
     static constexpr uint32_t TMEM_A = 4 * SG_T;
+    // at D = 64 there is room for X and Y behind the sums, two 16-bit elements per column
+    static constexpr bool ROWS_IN_TMEM = D == 64;
+    static constexpr uint32_t TMEM_X = TMEM_A + 2 * D, TMEM_Y = TMEM_X + D / 2;
     static_assert(SMEM <= 232448, "shared memory budget exceeded");
-    static_assert(TMEM_A + 2 * D <= TMEM_COLS, "TMEM budget exceeded");
+    static_assert(TMEM_A + 2 * D + (ROWS_IN_TMEM ? D : 0) <= TMEM_COLS, "TMEM budget exceeded");
 };
 
 // 16-byte aligned untiled copy global -> shared, counted on `bar`
@@ -233,6 +237,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
     const uint32_t empty = smem_u32(bars + 5);       // [4]
     const uint32_t s_full = smem_u32(bars + 9);      // [2]  S_j and dP_j are complete in TMEM (and with them every product issued before)
     const uint32_t a_ready = smem_u32(bars + 11);    // [2]  S_j and dP_j have been read, P_j and dx_j are in TMEM
+    const uint32_t xy_tmem = smem_u32(bars + 13);    // X and Y are in TMEM (D = 64)
     const uint32_t sums_done = smem_u32(bars + 15);
     const uint32_t drain_bar = smem_u32(bars + 16);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 18);
@@ -283,6 +288,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             mbar_init(s_full + 8 * g, 1);
             mbar_init(a_ready + 8 * g, 8);           // one arrival per warp of the group
         }
+        mbar_init(xy_tmem, 16);                      // one arrival per warp
         mbar_init(sums_done, 1);
         mbar_init(drain_bar, 1);
         *abort_flag = 0u;
@@ -362,6 +368,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         bool issued_any = false;
         if (ok) {
             bool w = att_wait(xy_full, 0u, wctx, 0x51000000u);
+            if (w && Cfg::ROWS_IN_TMEM) w = att_wait(xy_tmem, 0u, wctx, 0x53000000u);
             ok = __all_sync(0xFFFFFFFFu, w);
         }
         auto score_mmas = [&](int j) {
@@ -373,14 +380,16 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
                 const uint32_t a_off = (t >> 2) * (ATT_BM * 128) + (t & 3) * 32, b_off = (t >> 2) * (SG_T * 128) + (t & 3) * 32;
                 const uint64_t a_desc = desc_hi | ((((x_smem + a_off) >> 4) & 0x3FFFu) | lbo_k);
                 const uint64_t b_desc = desc_hi | ((((u_smem + b_off) >> 4) & 0x3FFFu) | lbo_k);
-                umma_ss<KIND_F16, 1>(s_tmem, a_desc, b_desc, idesc_s, t != 0 ? 1u : 0u);
+                if constexpr (Cfg::ROWS_IN_TMEM) umma_ts_f16(s_tmem, tmem_base + Cfg::TMEM_X + t * 8, b_desc, idesc_s, t != 0 ? 1u : 0u);
+                else umma_ss<KIND_F16, 1>(s_tmem, a_desc, b_desc, idesc_s, t != 0 ? 1u : 0u);
             }
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
                 const uint32_t a_off = (t >> 2) * (ATT_BM * 128) + (t & 3) * 32, b_off = (t >> 2) * (SG_T * 128) + (t & 3) * 32;
                 const uint64_t a_desc = desc_hi | ((((y_smem + a_off) >> 4) & 0x3FFFu) | lbo_k);
                 const uint64_t b_desc = desc_hi | ((((w_smem + b_off) >> 4) & 0x3FFFu) | lbo_k);
-                umma_ss<KIND_F16, 1>(s_tmem + SG_T, a_desc, b_desc, idesc_s, t != 0 ? 1u : 0u);
+                if constexpr (Cfg::ROWS_IN_TMEM) umma_ts_f16(s_tmem + SG_T, tmem_base + Cfg::TMEM_Y + t * 8, b_desc, idesc_s, t != 0 ? 1u : 0u);
+                else umma_ss<KIND_F16, 1>(s_tmem + SG_T, a_desc, b_desc, idesc_s, t != 0 ? 1u : 0u);
             }
             umma_commit<1>(s_full + 8 * g);
         };
@@ -496,6 +505,30 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
         }
         int t = t_first, head = head0;
         bool ok = true;
+        if constexpr (Cfg::ROWS_IN_TMEM) {
+            // X (group 0) and Y (group 1) go from shared memory to TMEM, half a row per thread, and are the scores' A operands there
+            if (n_tiles > 0) {
+                ok = att_wait(xy_full, 0u, wctx, 0x63000000u);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (ok) {
+                    uint32_t v[16];
+                    const uint8_t* src = smem + g * Cfg::X_BYTES + row * 128;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(src + (((half * 4 + c) ^ (row & 7)) << 4));
+                        v[4 * c] = x.x;
+                        v[4 * c + 1] = x.y;
+                        v[4 * c + 2] = x.z;
+                        v[4 * c + 3] = x.w;
+                    }
+                    tmem_st_32x32(t_lane + (g == 0 ? Cfg::TMEM_X : Cfg::TMEM_Y) + half * 16, v);
+                    tmem_st_wait();
+                    tcgen05_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(xy_tmem);
+                }
+            }
+        }
         auto next_tile = [&]() {
             if (++t == per_head) {
                 t = 0;
@@ -503,7 +536,7 @@ sm120_score_attention_grad_kernel(const __grid_constant__ CUtensorMap tmap_x,
             }
         };
         if (g == 1 && n_tiles > 0) next_tile();
-        for (int j = g; j < n_tiles; j += 2) {
+        for (int j = g; ok && j < n_tiles; j += 2) {
             const uint32_t st = j % SG_STAGES;
             const int u0 = tile_start(u_lo, t);
             const uint8_t* stat = smem + Cfg::STAT_OFF + st * Cfg::STAT_BYTES;
