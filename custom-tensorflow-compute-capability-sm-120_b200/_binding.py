@@ -96,8 +96,10 @@ class SM120ScoreAttentionDesc(Structure):
     ]
 
 
-# the same layout for callers that fill all fields at once: one struct.pack instead of some forty attribute stores (about 10 us of host time)
+# the same layout for callers that fill all fields at once: one struct.pack instead of some forty attribute stores (about 10 us of host time);
+# the last three fields (workspace, its size, stream) by themselves
 SCORE_ATTENTION_PACK = struct.Struct("@Iiii6q2f8P12q4P12q3Pq4qPQP")
+SCORE_ATTENTION_TAIL = struct.Struct("@PQP")
 
 
 # name -> (restype, argtypes): every symbol the public header declares
@@ -190,6 +192,18 @@ def new_score_attention_desc() -> SM120ScoreAttentionDesc:
     d = SM120ScoreAttentionDesc()
     load_library().sm120_score_attention_desc_init(ctypes.byref(d))
     return d
+
+
+_score_attention_calls: dict = {}
+
+
+def score_attention_call(name: str):
+    """The entry point `name` taking a packed SM120ScoreAttentionDesc as bytes."""
+    fn = _score_attention_calls.get(name)
+    if fn is None:
+        fn = ctypes.CFUNCTYPE(EXPORTS[name][0], c_char_p)((name, load_library()))
+        _score_attention_calls[name] = fn
+    return fn
 
 
 def error_string(code: int) -> str:

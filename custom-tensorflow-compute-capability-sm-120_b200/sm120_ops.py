@@ -880,35 +880,39 @@ def _score_scalars(dim: int, scale: Optional[float], softcap: Optional[float]):
     return scale, float(softcap)
 
 
-def _score_desc(*fields) -> _b.SM120ScoreAttentionDesc:
-    return _b.SM120ScoreAttentionDesc.from_buffer(bytearray(_b.SCORE_ATTENTION_PACK.pack(_b.SCORE_ATTENTION_PACK.size, *fields)))
+def _score_desc(*fields) -> bytes:
+    """The descriptor's bytes: packed at once and passed as they are (``_binding.score_attention_call``), which saves a few us of host time per call."""
+    return _b.SCORE_ATTENTION_PACK.pack(_b.SCORE_ATTENTION_PACK.size, *fields)
 
 
-def _score_launch(entry, what: str, d, index: int) -> None:
+def _score_launch(entry: str, what: str, desc: bytes, index: int) -> None:
     """Calls a descriptor-taking entry point with the device of the tensors current; its stream is already in the descriptor."""
+    fn = _b.score_attention_call(entry)
     if index == torch.cuda.current_device():
-        rc = entry(ctypes.byref(d))
+        rc = fn(desc)
     else:
         with torch.cuda.device(index):
-            rc = entry(ctypes.byref(d))
+            rc = fn(desc)
     if rc == _b.CUDA_ERROR_INVALID_VALUE:
         raise InvalidArgumentError(f"{what} rejected its arguments (cudaErrorInvalidValue)")
     if rc != _b.CUDA_SUCCESS:
         raise InternalError(f"{what} failed: {_b.error_string(rc)}")
 
 
-def _score_workspace(entry, d, index: int) -> Optional[torch.Tensor]:
-    """Scratch from the caller's allocator for this call alone: two captured graphs, or two streams, never share it."""
+def _score_workspace(entry: str, desc: bytes, like: torch.Tensor, index: int):
+    """(descriptor, scratch): scratch comes from the caller's allocator for this call alone: two captured graphs, or two streams,
+    never share it.  The caller holds it until the launch is queued."""
+    fn = _b.score_attention_call(entry)
     if index == torch.cuda.current_device():
-        need = int(entry(ctypes.byref(d)))
+        need = fn(desc)
     else:
         with torch.cuda.device(index):
-            need = int(entry(ctypes.byref(d)))
+            need = fn(desc)
     if not need:
-        return None
-    ws = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
-    d.workspace, d.workspace_bytes = ws.data_ptr(), need
-    return ws
+        return desc, None
+    ws = like.new_empty(need, dtype=torch.uint8)
+    tail = _b.SCORE_ATTENTION_TAIL
+    return desc[:-tail.size] + tail.pack(ws.data_ptr(), need, _raw_stream(index)), ws
 
 
 def _score_out(out: Optional[torch.Tensor], query: torch.Tensor) -> torch.Tensor:
@@ -1002,10 +1006,10 @@ def score_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     query, key, value, head, side = _score_sequence(query, key, value, scale, causal_mask, softcap, alibi_slopes, document_offsets, prefix_lengths)
     out = _score_out(out, query)
     index = query.get_device()
-    lse = torch.empty(query.shape[:3], dtype=torch.float32, device=query.device) if return_lse else None
+    lse = query.new_empty(query.shape[:3], dtype=torch.float32) if return_lse else None
     d = _score_desc(*head, out.data_ptr(), lse.data_ptr() if return_lse else 0, *side, *query.stride()[:3], *key.stride()[:3], *value.stride()[:3],
                     *out.stride()[:3], 0, 0, 0, 0, *_ZERO3, *_ZERO3, *_ZERO3, *_ZERO3, 0, 0, 0, 0, *_ZERO2, *_ZERO2, 0, 0, _raw_stream(index))
-    _score_launch(_b.load_library().sm120_launch_score_attention, "score_attention", d, index)
+    _score_launch("sm120_launch_score_attention", "score_attention", d, index)
     return (out, lse) if return_lse else out
 
 
@@ -1025,12 +1029,12 @@ def score_attention_grad(grad_out: torch.Tensor, query: torch.Tensor, key: torch
                                                     grad_out, out, lse)
     out, grad_out = _score_operand(out), _score_operand(grad_out)
     dq, dk, dv = torch.empty_like(query), torch.empty_like(key), torch.empty_like(value)
-    index, lib = query.get_device(), _b.load_library()
+    index = query.get_device()
     d = _score_desc(*head, out.data_ptr(), lse.data_ptr(), *side, *query.stride()[:3], *key.stride()[:3], *value.stride()[:3], *out.stride()[:3],
                     grad_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *grad_out.stride()[:3], *dq.stride()[:3],
                     *dk.stride()[:3], *dv.stride()[:3], 0, 0, 0, 0, *_ZERO2, *_ZERO2, 0, 0, _raw_stream(index))
-    ws = _score_workspace(lib.sm120_score_attention_grad_workspace_bytes, d, index)      # held until the launch is queued
-    _score_launch(lib.sm120_launch_score_attention_grad, "score_attention_grad", d, index)
+    d, ws = _score_workspace("sm120_score_attention_grad_workspace_bytes", d, query, index)
+    _score_launch("sm120_launch_score_attention_grad", "score_attention_grad", d, index)
     del ws
     return dq, dk, dv
 
@@ -1096,15 +1100,15 @@ def _score_token(what: str, query, prefix_key, prefix_value, key_cache, value_ca
         prefix_key, prefix_value = _score_operand(prefix_key), _score_operand(prefix_value)
         tail = (prefix_key.data_ptr(), prefix_value.data_ptr(), prefix, *prefix_key.stride()[:2], *prefix_value.stride()[:2])
     out = _score_out(out, query)
-    index, lib = query.get_device(), _b.load_library()
-    lse = torch.empty((b, h), dtype=torch.float32, device=query.device) if return_lse else None
+    index = query.get_device()
+    lse = query.new_empty((b, h), dtype=torch.float32) if return_lse else None
     d = _score_desc(_TORCH_TO_SM120[query.dtype], 0, 0, b, h, kv_heads, 1, sk, dim, scale, softcap, query.data_ptr(), key_cache.data_ptr(),
                     value_cache.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
                     0 if alibi_slopes is None else alibi_slopes.data_ptr(), 0, 0, *query.stride()[:2], 0, *key_cache.stride()[:3],
                     *value_cache.stride()[:3], *out.stride()[:2], 0, 0, 0, 0, 0, *_ZERO3, *_ZERO3, *_ZERO3, *_ZERO3, lengths.data_ptr(), *tail,
                     0, 0, _raw_stream(index))
-    ws = _score_workspace(lib.sm120_score_attention_decode_workspace_bytes, d, index)    # held until the launch is queued
-    _score_launch(lib.sm120_launch_score_attention_decode, what, d, index)
+    d, ws = _score_workspace("sm120_score_attention_decode_workspace_bytes", d, query, index)
+    _score_launch("sm120_launch_score_attention_decode", what, d, index)
     del ws
     return (out, lse) if return_lse else out
 

@@ -143,6 +143,15 @@ def test_packed_descriptor_has_the_structs_layout(binding):
         assert (list(got) if isinstance(want, list) else got) == want, name
 
 
+def test_packed_descriptor_reaches_the_entry_points(binding):
+    d = _good(binding, "grad")
+    d.workspace, d.workspace_bytes = None, 0
+    packed = bytes(d)
+    assert packed[-binding.SCORE_ATTENTION_TAIL.size:] == binding.SCORE_ATTENTION_TAIL.pack(0, 0, 0)
+    assert binding.score_attention_call(LAUNCH["grad"])(packed) == 1              # no workspace
+    assert binding.score_attention_call(LAUNCH["forward"])(b"\0" * len(packed)) == 1
+
+
 def test_needs_a_gpu(ops):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
