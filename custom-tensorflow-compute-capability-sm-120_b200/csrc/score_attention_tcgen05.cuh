@@ -218,6 +218,9 @@ sm120_score_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
     volatile int* xseq = reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(bars) + 256 + 2 * 2 * ATT_BM * 4);   // [2][ATT_BM]
     if (threadIdx.x < 2 * ATT_BM) xseq[threadIdx.x] = 0;
 
+    // the caches' launch behind this one reads nothing that this one writes: it may begin as soon as all blocks here have
+    if (TOKEN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const ScoreParams& sp = p.s;

@@ -443,6 +443,47 @@ def test_large_batches_behind_a_shared_prefix(ops, prefix):
         token_and_check(ops, gen, dtype, b, h, hk, 70, d, [(13 * e) % 71 for e in range(b)], prefix, 20.0 if d == 64 else None, True)
 
 
+def test_prefix_and_caches_overlap_in_order(ops):
+    """The caches' launch may begin while the prefix's still runs: results stay those of the ordered calls, back to back on changing
+    inputs, on two streams and in a replayed graph, and what is queued behind sees them complete."""
+    gen = torch.Generator(device="cuda").manual_seed(45)
+    b, h, hk, d, p, s = 64, 16, 4, 128, 9000, 900
+    sets = []
+    for _ in range(3):
+        q = normal(gen, b, h, d, dtype=torch.bfloat16)
+        pk, pv = (normal(gen, hk, p, d, dtype=torch.bfloat16) for _ in range(2))
+        k, v = (normal(gen, b, hk, s, d, dtype=torch.bfloat16) for _ in range(2))
+        sets.append((q, pk, pv, k, v, torch.randint(0, s + 1, (b,), generator=gen, device="cuda").int()))
+    sets[2][5].zero_()                                                 # no request has keys of its own: the caches' blocks end at once
+    want = []
+    for args in sets:
+        torch.cuda.synchronize()
+        want.append(ops.shared_prefix_attention(*args).clone())
+        torch.cuda.synchronize()
+    ref_out = ref.token_attention(*[sets[0][i] for i in (0, 3, 4)], sets[0][5].tolist(), prefix_k=sets[0][1], prefix_v=sets[0][2])
+    within(want[0], ref_out["out"], ref_out["out_tol"], "overlap")
+    for _ in range(10):
+        got = [ops.shared_prefix_attention(*args).float() * 2 for args in sets for _ in range(2)]
+        assert all(torch.equal(g, want[i // 2].float() * 2) for i, g in enumerate(got))
+    static = [t.clone() for t in sets[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = ops.shared_prefix_attention(*static).float() * 2
+    for turn in range(6):
+        for t, src in zip(static, sets[turn % 3]):
+            t.copy_(src)
+        graph.replay()
+        assert torch.equal(res, want[turn % 3].float() * 2), turn
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ops.shared_prefix_attention(*sets[i % 3]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(outs))
+
+
 def test_prefix_form_equals_the_cache_form(ops):
     """The same keys as one cache and as prefix + cache give the same result up to the join's rounding; no prefix is the cache form itself."""
     gen = torch.Generator(device="cuda").manual_seed(41)
